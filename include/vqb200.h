@@ -570,6 +570,83 @@ typedef struct vq_skvq_dequant_args {
 } vq_skvq_dequant_args;
 int32_t vq_skvq_unpack_dequant(const vq_skvq_dequant_args *args, void *stream);
 
+/* ------------------------------------------------------------------------------------
+ * Rotary positions (no counterpart in the reference, whose models rotate before they reach it)
+ * ---------------------------------------------------------------------------------- */
+/* Up to two tensors are rotated and a third is copied, in one launch. Every tensor i is
+ * [B, heads[i], S, D] with its channels contiguous; x[i] NULL = absent. Of each head the first
+ * rotary_dim channels form pairs: (c, c + rotary_dim/2) in the half layout (0), (2c, 2c + 1) in the
+ * interleaved layout (1); pair c of the token at position p is turned by t = turns[c] * p full
+ * turns, y = factor * (a cos t - b sin t, b cos t + a sin t), inverse != 0: by -t (with the same
+ * factor: the gradient). Channels from rotary_dim on are copied. turns is float64 (frequency /
+ * 2 pi): the product is taken and reduced to one turn in 64 bits, sine and cosine in 32.
+ * Position of token (b, s): pos_offset + positions[b*pos_stride_b + s*pos_stride_s], or
+ * pos_offset + s when positions is NULL. Outputs must not overlap inputs.
+ * Used with y[1] / y[2] behind the residual window of a KIVI cache it is the append of a decode
+ * step: rotated queries out, rotated keys and the values into the cache (see vq_kivi_append). */
+typedef struct vq_rotary_args {
+    const void *x[3];         /* 0, 1 rotated; 2 copied */
+    void *y[3];
+    int64_t x_stride[3][3];   /* elements between batch elements, heads, tokens */
+    int64_t y_stride[3][3];
+    int32_t heads[3];
+    int32_t dtype;            /* vq_dtype of all tensors */
+    int64_t B, S;
+    int32_t D, rotary_dim;    /* 2 <= rotary_dim <= D, even */
+    int32_t layout, inverse;
+    const void *positions;    /* int32 or int64, or NULL */
+    int32_t pos_bytes;        /* 4 or 8 */
+    float factor;
+    int64_t pos_stride_b, pos_stride_s, pos_offset;
+    const double *turns;      /* [rotary_dim/2] */
+} vq_rotary_args;
+int32_t vq_rotary(const vq_rotary_args *args, void *stream);
+
+/* ------------------------------------------------------------------------------------
+ * Attention of a batch that shares a prefix (no counterpart in the reference)
+ * ---------------------------------------------------------------------------------- */
+/* Packed KIVI tokens and the exact rows behind them, of one batch element (the prefix) or of B. */
+typedef struct vq_kivi_rows {
+    const uint8_t *k_codes, *v_codes;           /* rows D*store_bits/8 bytes, 16-byte aligned */
+    const float *k_scale, *k_zero;              /* rows [token group][D] */
+    const float *v_scale, *v_zero;              /* rows [token][D/group] */
+    const void *k_res, *v_res;                  /* rows [token][D] in q's dtype, 16-byte aligned */
+    int64_t k_codes_stride_bh, v_codes_stride_bh; /* bytes between (batch, kv head) slabs */
+    int64_t k_param_stride_bh, v_param_stride_bh; /* floats */
+    int64_t res_stride_bh;                      /* elements */
+    int32_t n_quant;                            /* packed tokens, a multiple of group */
+    int32_t n_res;                              /* exact rows */
+} vq_kivi_rows;
+
+/* out[b, h, r] = softmax(scale * q[b, h, r] . [K_prefix | K_own[b]]) . [V_prefix | V_own[b]] with
+ * kv head h / (H_q/H_kv). The prefix is ONE store read by all B requests; every query row sees all
+ * of it. Own slot t of request b (packed tokens first, then the exact rows; n = n_quant + n_res of
+ * `own`) is seen by query row r when t >= own_start[b] (NULL: 0; slots before it are padding) and,
+ * with VQ_ATTEND_CAUSAL, t <= n - S_q + r. A row that sees nothing gives zeros (and lse -inf).
+ * float16 or bfloat16; D 64 or 128, group 32, store_bits 2, 4 or 8. Decoded keys and values
+ * enter the tensor cores as float16 (also for bfloat16 queries), so code*scale+zero, the exact
+ * rows and q must lie within +-65504. */
+typedef struct vq_shared_attend_args {
+    const void *q;            /* [B, H_q, S_q, D] contiguous */
+    void *out;                /* [B, H_q, S_q, D] contiguous, dtype of q */
+    float *lse;               /* [B, H_q, S_q] natural log of the softmax sum, or NULL */
+    const int32_t *own_start; /* [B] or NULL */
+    int32_t dtype;            /* VQ_F16 or VQ_BF16 */
+    int32_t B, H_q, H_kv, S_q, D;
+    int32_t store_bits, group;
+    float scale;
+    int32_t flags;            /* 0 or VQ_ATTEND_CAUSAL */
+    vq_kivi_rows prefix, own;
+    void *workspace;          /* >= vq_kivi_shared_attend_workspace_bytes(args), 16-byte aligned */
+    int64_t workspace_bytes;
+    int32_t variant;          /* 0 = choose; 1 = warp tiles for the prefix too; 2 = the tcgen05 kernel
+                                 for the prefix */
+    int32_t n_splits;         /* context splits of the prefix; 0 = choose */
+} vq_shared_attend_args;
+int64_t vq_kivi_shared_attend_workspace_bytes(const vq_shared_attend_args *args);
+/* vq_kivi_attend_status also reports the bounded waits of this call's kernels. */
+int32_t vq_kivi_shared_attend(const vq_shared_attend_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -153,6 +153,36 @@ class SkvqDequantArgs(C.Structure):
     ]
 
 
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p * 3), ("y", C.c_void_p * 3), ("x_stride", C.c_int64 * 9), ("y_stride", C.c_int64 * 9),
+        ("heads", C.c_int32 * 3), ("dtype", C.c_int32), ("B", C.c_int64), ("S", C.c_int64),
+        ("D", C.c_int32), ("rotary_dim", C.c_int32), ("layout", C.c_int32), ("inverse", C.c_int32),
+        ("positions", C.c_void_p), ("pos_bytes", C.c_int32), ("factor", C.c_float),
+        ("pos_stride_b", C.c_int64), ("pos_stride_s", C.c_int64), ("pos_offset", C.c_int64), ("turns", C.c_void_p),
+    ]
+
+
+class KiviRowsArgs(C.Structure):
+    _fields_ = [
+        ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scale", C.c_void_p), ("k_zero", C.c_void_p),
+        ("v_scale", C.c_void_p), ("v_zero", C.c_void_p), ("k_res", C.c_void_p), ("v_res", C.c_void_p),
+        ("k_codes_stride_bh", C.c_int64), ("v_codes_stride_bh", C.c_int64),
+        ("k_param_stride_bh", C.c_int64), ("v_param_stride_bh", C.c_int64), ("res_stride_bh", C.c_int64),
+        ("n_quant", C.c_int32), ("n_res", C.c_int32),
+    ]
+
+
+class SharedAttendArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("own_start", C.c_void_p), ("dtype", C.c_int32),
+        ("B", C.c_int32), ("H_q", C.c_int32), ("H_kv", C.c_int32), ("S_q", C.c_int32), ("D", C.c_int32),
+        ("store_bits", C.c_int32), ("group", C.c_int32), ("scale", C.c_float), ("flags", C.c_int32),
+        ("prefix", KiviRowsArgs), ("own", KiviRowsArgs),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("variant", C.c_int32), ("n_splits", C.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/vqb200.h declares.
 SIGNATURES = {
     "vq_version": (C.c_int32, []),
@@ -202,6 +232,9 @@ SIGNATURES = {
                                          C.c_int32, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),
     "vq_skvq_quantize_pack": (C.c_int32, [C.POINTER(SkvqQuantArgs), C.c_void_p]),
     "vq_skvq_unpack_dequant": (C.c_int32, [C.POINTER(SkvqDequantArgs), C.c_void_p]),
+    "vq_rotary": (C.c_int32, [C.POINTER(RotaryArgs), C.c_void_p]),
+    "vq_kivi_shared_attend_workspace_bytes": (C.c_int64, [C.POINTER(SharedAttendArgs)]),
+    "vq_kivi_shared_attend": (C.c_int32, [C.POINTER(SharedAttendArgs), C.c_void_p]),
     "vq_bit_pack": (C.c_int32, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p]),
     "vq_bit_unpack": (C.c_int32, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p]),
 }

@@ -40,6 +40,8 @@ SOURCES = [
     ("rabitq_prefill.cu", []),
     ("rvq.cu", []),
     ("skvq.cu", ["-fmad=false"]),
+    ("rotary.cu", []),
+    ("shared_attend.cu", []),
 ]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -505,6 +505,8 @@ class KIVIKVCache(StandaloneProtocol):
     token-by-token decode quantize identical groups. Never exposes ``.bits``.
     """
 
+    _rollbacks = 0   # trims, resets and reloads so far: rows that a fork of this cache refers to may be rewritten after one
+
     def __init__(self, config: Any) -> None:
         _native_only(config, "KIVIKVCache")
         self._head_dim = int(config.head_dim)
@@ -697,6 +699,10 @@ class KIVIKVCache(StandaloneProtocol):
             if self._memory_bound:
                 return self._sentinel, self._sentinel
             return self._materialize()
+        return self._append_block(keys, values, overlap_previous, self._store_block)
+
+    def _append_block(self, keys, values, overlap_previous, store):
+        """``store(keys, values, S, overlap_previous)`` puts a block behind the live residual rows."""
         if keys.ndim != 4 or keys.shape != values.shape:
             raise ValueError(f"KIVIKVCache.update_and_fetch: keys/values must be equal 4D shapes, got "
                              f"{tuple(keys.shape)} / {tuple(values.shape)}")
@@ -713,7 +719,7 @@ class KIVIKVCache(StandaloneProtocol):
         self._just_flushed = n_flush > 0
         if n_flush <= 0:
             self._make_room(B, H, D, S, dev, keys.dtype)
-            self._store_block(keys, values, S, overlap_previous)
+            store(keys, values, S, overlap_previous)
         elif self._n_res == 0:
             # A (prefill) block onto an empty residual: its head is quantized straight from the
             # caller's tensor, only its tail is copied into the residual buffer.
@@ -730,7 +736,7 @@ class KIVIKVCache(StandaloneProtocol):
             # the live rows, then the aged rows are quantized where they lie and the window's
             # start moves on: no concatenation, no shifting, no allocation.
             self._make_room(B, H, D, S, dev, keys.dtype)
-            self._store_block(keys, values, S)
+            store(keys, values, S, False)
             self._ensure_capacity(B, H, D, new_boundary, dev, keys.dtype)
             lo = self._res_lo
             self._quantize_rows(self._k_res[:, :, lo : lo + n_flush], self._v_res[:, :, lo : lo + n_flush], n_flush)
@@ -764,6 +770,33 @@ class KIVIKVCache(StandaloneProtocol):
                 self._sentinel = keys.new_zeros((B, H, 0, D))
             return self._sentinel, self._sentinel
         return self._materialize()
+
+    def update_rotary(self, q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, rope: Any, positions=None):
+        """Rotate ``q [B,H_q,S,D]`` and ``keys [B,H_kv,S,D]`` with ``rope`` (a
+        :class:`rotary.RotaryEmbedding`) and append the rotated keys and ``values``: ``(rotated q,
+        *update_and_fetch(rotated keys, values))``. ``positions``: as in the embedding; by default the
+        tokens follow the cached ones. A block that goes through the residual window (every decode
+        step) is rotated straight into it, in one launch; a prompt is rotated first."""
+        if positions is None:
+            positions = int(self.offset)
+        if (type(self).update_and_fetch is KIVIKVCache.update_and_fetch and q.ndim == 4 and keys.ndim == 4 and keys.shape == values.shape
+                and keys.shape[3] == self._head_dim and (self._k_res is None or (self._k_res.dtype is keys.dtype and self._k_res.device == keys.device
+                                                                                  and self._k_res.shape[:2] == keys.shape[:2]))):
+            S, g = keys.shape[2], self._group_size
+            aged = max(0, self.offset + S - self._residual_length) // g * g > self._n_quantized
+            if S and (not aged or (self._n_res and S <= self._residual_length + g)):
+                rope._check_append(q, keys, values)   # (before the cache's counters move)
+                rope._positions("KIVIKVCache.update_rotary", positions, keys.shape[0], S, keys.device)
+                turned = []
+
+                def store(k, v, n, _overlap):
+                    turned.append(rope.append(q, k, v, self._k_res, self._v_res, self._res_lo + self._n_res, positions))
+                    self._n_res += n
+
+                out = self._append_block(keys, values, False, store)
+                return (turned[0], *out)
+        q2, k2 = rope(q, keys, positions)
+        return (q2, *self.update_and_fetch(k2, values))
 
     def _live_res(self):
         lo = self._res_lo
@@ -873,6 +906,7 @@ class KIVIKVCache(StandaloneProtocol):
         n = int(min(max(n, 0), self.offset))
         if n == 0:
             return 0
+        self._rollbacks += 1
         new_offset = self.offset - n
         g = self._group_size
         old_nq = self._n_quantized
@@ -916,6 +950,7 @@ class KIVIKVCache(StandaloneProtocol):
 
     def _reset_tokens(self) -> None:
         """Forget every token; buffers, bit-width and group size stay (``KVCache.reset``)."""
+        self._rollbacks += 1
         self.offset = self._n_quantized = self._n_res = self._res_lo = 0
         self._key_bytes_compressed = self._value_bytes_compressed = 0
         self._key_bytes_fp16 = self._value_bytes_fp16 = self._residual_fp16_bytes = self._tokens_seen = 0
@@ -937,6 +972,7 @@ class KIVIKVCache(StandaloneProtocol):
         if not st:
             return
         kc, ks, kz, vc, vs, vz, kr, vr, counters = st
+        self._rollbacks += 1
         self.offset, nq, n_res = (int(x) for x in counters.tolist())
         B, H, _, D = kr.shape
         self._shape_bhd, self._dtype = (B, H, D), kr.dtype

@@ -1,0 +1,66 @@
+// Internal interface between the shared-prefix attention's entry point and its prefix kernel.
+#pragma once
+#include "common.cuh"
+
+namespace vq {
+
+// Partial softmax records in the workspace: of output row r and split j of n_splits,
+//   o  [(r * n_splits + j) * D + d]  sum over the split's slots of 2^(score - m) * v
+//   ml [(r * n_splits + j) * 2]      m (maximum score in the base-2 domain, -inf: nothing seen) and l
+struct SharedPartials {
+    float *o, *ml;
+    int n_splits;  // prefix splits, then own splits
+};
+
+// Whether the tcgen05 kernel takes the prefix of `a` (NULL) or why not, the splits it would use, its
+// launch into splits [0, np) of `parts`, and its "a bounded wait gave up" flag.
+const char *shared_prefix_tc5_supported(const vq_shared_attend_args &a);
+int shared_prefix_tc5_splits(const vq_shared_attend_args &a, const DeviceInfo &di);
+int32_t shared_prefix_tc5_launch(const vq_shared_attend_args &a, const SharedPartials &parts, int np, const DeviceInfo &di, cudaStream_t st);
+int32_t shared_prefix_tc5_take_timeout(int *flag);
+
+// ---- packed codes to numbers ------------------------------------------------------------------
+// A code c becomes the float BASE + c by placing its byte into the mantissa of BASE (one byte
+// permutation), and code*scale + zero becomes one fused multiply-add against zero - BASE*scale.
+// That difference is rounded once: an error of at most 2^-24 * BASE * scale, 2^-17 (2- and 4-bit
+// codes) or 2^-9 (8-bit) of the quantization step.
+template <int SB>
+struct Codes {
+    static constexpr float kBase = SB == 8 ? 32768.f : 128.f;
+    static constexpr int kPerWord = 32 / SB;
+    // Codes i of `w` whose index is a multiple of 8/SB ... shifted so that each sits alone in its byte.
+    __device__ static __forceinline__ uint32_t plane(uint32_t w, int k) {
+        if constexpr (SB == 8) return w;
+        else return (w >> (SB * k)) & (SB == 4 ? 0x0f0f0f0fu : 0x03030303u);
+    }
+    // BASE + the code in byte `b` of a plane
+    __device__ static __forceinline__ float place(uint32_t plane, int b) {
+        if constexpr (SB == 8) return __uint_as_float(__byte_perm(plane, 0x47000000u, 0x7404u | ((uint32_t)b << 4)));
+        else return __uint_as_float(__byte_perm(plane, 0x43000000u, 0x7044u | ((uint32_t)b << 8)));
+    }
+    // code i of word w (i a compile-time constant after unrolling)
+    __device__ static __forceinline__ float get(uint32_t w, int i) { return place(plane(w, i % (8 / SB)), i / (8 / SB)); }
+};
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two neighbouring 16-bit floats as packed halves (bfloat16 goes through float32: exact inside
+// half's normal range)
+template <typename T>
+__device__ __forceinline__ uint32_t as_f16x2(uint32_t raw);
+template <>
+__device__ __forceinline__ uint32_t as_f16x2<__half>(uint32_t raw) { return raw; }
+template <>
+__device__ __forceinline__ uint32_t as_f16x2<__nv_bfloat16>(uint32_t raw) {
+    return pack_f16(__uint_as_float(raw << 16), __uint_as_float(raw & 0xffff0000u));
+}
+
+}  // namespace vq

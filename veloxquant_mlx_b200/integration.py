@@ -212,6 +212,19 @@ def make_hf_cache(model_or_n_layers: Any, config: KVCacheConfig):
     return Cache(layers=[Layer(c) for c in caches])
 
 
+def fork_hf_cache(cache: Any, batch: int):
+    """A ``transformers.Cache`` for ``batch`` requests that continue one prefilled prompt: ``cache`` is a
+    cache of :func:`make_hf_cache` (method ``kivi``) after the prompt ran through the model at batch 1.
+    Its layers' packed prompt is shared, not copied; every layer of the result is a
+    ``shared_prefix.SharedPrefixKIVICache`` (attend with :func:`veloxquant_attention`)."""
+    from transformers.cache_utils import Cache
+
+    from .shared_prefix import SharedPrefixKIVICache
+
+    Layer = make_cache_layer_class()
+    return Cache(layers=[Layer(SharedPrefixKIVICache(layer.cache, batch)) for layer in cache.layers])
+
+
 def patch_model_kv_cache(model: Any, config: KVCacheConfig):
     """Give ``model`` a ``make_cache()`` hook that builds a FRESH compressed cache on every call
     (``model.generate(..., past_key_values=model.make_cache())``), and return the first one,
@@ -273,5 +286,5 @@ def patch_hf_for_fused_sdpa(model: Any, name: str = "veloxquant") -> None:
             cfg._attn_implementation = name
 
 
-__all__ = ["fused_sdpa_dispatch", "make_hf_cache", "patch_model_kv_cache", "veloxquant_attention", "register_attention",
+__all__ = ["fused_sdpa_dispatch", "make_hf_cache", "fork_hf_cache", "patch_model_kv_cache", "veloxquant_attention", "register_attention",
            "patch_hf_for_fused_sdpa", "make_cache_layer_class"]

@@ -690,6 +690,7 @@ _DEFINED_ELSEWHERE = {
     "vecinfer_quantize_metal": "vecinfer", "vecinfer_dequant_metal": "vecinfer",
     "vecinfer_encode_decode_metal": "vecinfer", "vecinfer_encode_decode_simple_metal": "vecinfer",
     "metal_fused_sdpa": "vecinfer",
+    "KiviRows": "shared_prefix", "kivi_shared_prefix_attend": "shared_prefix",
 }
 
 
@@ -699,7 +700,8 @@ def __getattr__(name: str):
         raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
     import importlib
 
-    return getattr(importlib.import_module("." + module, __package__), name)
+    value = globals()[name] = getattr(importlib.import_module("." + module, __package__), name)
+    return value
 
 
 __all__ = [

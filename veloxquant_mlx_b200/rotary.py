@@ -1,0 +1,291 @@
+"""Rotary positions: the step between a layer's projections and its cache.
+
+``RotaryEmbedding`` holds the frequencies of one model and turns queries and keys in one launch
+(half or interleaved layout, all or part of the head, frequencies scaled for long contexts).
+It is differentiable: the gradient is the inverse turn. :meth:`RotaryEmbedding.append` is the
+form of a decode step: rotated queries out, rotated keys and the values straight behind the
+unquantized window of a KIVI cache (used by ``KIVIKVCache.update_rotary``).
+
+The reference has no counterpart: its caches receive keys that the model has rotated.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Any
+
+import torch
+
+from . import _lib
+from ._lib import RotaryArgs, check, dtype_code, lib, require_cuda, stream_ptr
+
+_LAYOUTS = ("half", "interleaved")
+_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None) -> tuple[torch.Tensor, float]:
+    """Angle per position of each of the ``rotary_dim / 2`` pairs (float64, on the host) and the
+    factor on sine and cosine.
+
+    Without ``scaling``: ``base ** (-2 i / rotary_dim)`` and 1. ``scaling["rope_type"]`` is one of
+
+    * ``"default"``;
+    * ``"linear"``: every frequency divided by ``factor``;
+    * ``"ntk"``: ``base`` raised to ``base * factor ** (r / (r - 2))``, ``r = rotary_dim``;
+    * ``"llama3"``: wavelengths above ``original_max_position_embeddings / low_freq_factor`` are
+      stretched by ``factor``, those below ``.../ high_freq_factor`` are kept, a linear ramp (in the
+      number of turns over the original context) between;
+    * ``"yarn"``: the same between the pairs that make ``beta_slow`` (1) and ``beta_fast`` (32) turns
+      over the original context, the ramp linear in the pair's index (rounded outwards unless
+      ``truncate`` is false); the factor on sine and cosine is ``attention_factor``, by default
+      ``0.1 ln(factor) + 1``.
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_frequencies: rotary_dim={rotary_dim} must be even and at least 2")
+    if not base > 0:
+        raise ValueError(f"rotary_frequencies: base={base} must be positive")
+    pair = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    kind = "default" if not scaling else scaling.get("rope_type", scaling.get("type", "default"))
+    if kind not in ("default", "linear", "ntk", "llama3", "yarn"):
+        raise ValueError(f"rotary_frequencies: unknown rope_type {kind!r}")
+
+    def need(name):
+        if name not in scaling:
+            raise ValueError(f"rotary_frequencies: rope_type {kind!r} needs {name!r}")
+        return float(scaling[name])
+
+    if kind == "default":
+        return base ** (-2.0 * pair / rotary_dim), 1.0
+    factor = need("factor")
+    if not factor > 0:
+        raise ValueError(f"rotary_frequencies: factor={factor} must be positive")
+    if kind == "ntk":
+        if rotary_dim > 2:  # (a single pair turns by one radian a position whatever the base)
+            base = base * factor ** (rotary_dim / (rotary_dim - 2.0))
+        return base ** (-2.0 * pair / rotary_dim), 1.0
+    freq = base ** (-2.0 * pair / rotary_dim)
+    if kind == "linear":
+        return freq / factor, 1.0
+    old = need("original_max_position_embeddings")
+    if kind == "llama3":
+        lo, hi = need("low_freq_factor"), need("high_freq_factor")
+        if not hi > lo:
+            raise ValueError(f"rotary_frequencies: high_freq_factor={hi} must exceed low_freq_factor={lo}")
+        turns = old * freq / (2.0 * math.pi)
+        keep = ((turns - lo) / (hi - lo)).clamp(0.0, 1.0)
+        return freq * (keep + (1.0 - keep) / factor), 1.0
+    # yarn: the index of the pair that makes n turns over the original context
+    fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+    at = lambda n: rotary_dim * math.log(old / (n * 2.0 * math.pi)) / (2.0 * math.log(base))  # noqa: E731
+    lo, hi = at(fast), at(slow)
+    if scaling.get("truncate", True):
+        lo, hi = math.floor(lo), math.ceil(hi)
+    lo, hi = max(lo, 0), min(hi, rotary_dim - 1)
+    if hi == lo:
+        hi += 0.001
+    stretched = ((pair - lo) / (hi - lo)).clamp(0.0, 1.0)
+    att = scaling.get("attention_factor")
+    att = float(att) if att is not None else (0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0)
+    return freq * ((1.0 - stretched) + stretched / factor), att
+
+
+class RotaryEmbedding:
+    """The rotary positions of one model.
+
+    ``head_dim`` channels a head, of which the first ``rotary_dim`` (default: all) are turned, in
+    pairs ``(c, c + rotary_dim/2)`` (``layout="half"``) or ``(2c, 2c+1)`` (``"interleaved"``).
+    The frequencies are :func:`rotary_frequencies` of ``base`` and ``scaling``, or ``inv_freq``
+    (``[rotary_dim/2]``, angle per position, taken in float64); ``attention_factor`` overrides the
+    factor on sine and cosine.
+
+    ``rope(q, k, positions)`` returns the turned ``q`` and ``k`` (``rope(q)`` one tensor) as new
+    contiguous tensors: ``q [B, H_q, S, D]``, ``k [B, H_kv, S, D]`` in float16, bfloat16 or float32
+    with any strides (heads in the projection's ``[B, S, H, D]`` order included). ``positions`` is an
+    integer tensor ``[S]``, ``[1, S]`` or ``[B, S]`` on the same device, or an int: the position of token
+    0, the others following. ``inverse=True`` turns back. Products are float32, angles float64 (exact
+    to float32 for positions up to 2**31 and beyond); one rounding to the tensors' type at the end.
+    Gradients flow to ``q`` and ``k`` (also twice), not to positions or frequencies.
+
+    The frequency table is put on a device at its first use there; make that use (or pass
+    ``device=``) before a CUDA-graph capture.
+    """
+
+    def __init__(self, head_dim: int, *, rotary_dim: int | None = None, base: float = 10000.0, layout: str = "half",
+                 scaling: dict | None = None, inv_freq: Any = None, attention_factor: float | None = None, device=None) -> None:
+        rotary_dim = head_dim if rotary_dim is None else int(rotary_dim)
+        if head_dim < 2 or rotary_dim < 2 or rotary_dim > head_dim or rotary_dim % 2:
+            raise ValueError(f"RotaryEmbedding: rotary_dim={rotary_dim} must be even and in 2..head_dim={head_dim}")
+        if layout not in _LAYOUTS:
+            raise ValueError(f"RotaryEmbedding: layout must be one of {_LAYOUTS}, got {layout!r}")
+        if inv_freq is None:
+            freq, factor = rotary_frequencies(rotary_dim, base, scaling)
+        else:
+            if scaling is not None:
+                raise ValueError("RotaryEmbedding: give inv_freq or scaling, not both")
+            freq, factor = torch.as_tensor(inv_freq).detach().to("cpu", torch.float64), 1.0
+            if tuple(freq.shape) != (rotary_dim // 2,):
+                raise ValueError(f"RotaryEmbedding: inv_freq must have shape ({rotary_dim // 2},), got {tuple(freq.shape)}")
+        self.head_dim, self.rotary_dim, self.layout = int(head_dim), rotary_dim, layout
+        self.inv_freq = freq
+        self.attention_factor = float(factor if attention_factor is None else attention_factor)
+        self._turns_host = freq / (2.0 * math.pi)
+        self._turns: dict = {}
+        if device is not None:
+            self._turns_on(torch.device(device))
+
+    def _turns_on(self, device: torch.device) -> int:
+        """The table's address on ``device``."""
+        index = device.index if device.index is not None else torch.cuda.current_device()
+        t = self._turns.get(index)
+        if t is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("RotaryEmbedding: first use on a device inside a graph capture; pass device= or call it once before")
+            with _lib.on_device(device):
+                t = self._turns_host.to(torch.device("cuda", index))
+                torch.cuda.current_stream().synchronize()  # (any stream may read it from here on)
+            self._turns[index] = t
+        return t.data_ptr()
+
+    # -- checks --------------------------------------------------------------------------
+    def _check(self, fn, q, k):
+        for name, t in (("q", q), ("k", k)):
+            if t is None:
+                continue
+            if t.ndim != 4 or t.shape[3] != self.head_dim:
+                raise ValueError(f"{fn}: {name} must be [B, H, S, {self.head_dim}], got {tuple(t.shape)}")
+            if t.dtype not in _DTYPES:
+                raise ValueError(f"{fn}: unsupported dtype {t.dtype}; expected float16, bfloat16 or float32")
+        if k is not None and (k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.dtype is not q.dtype or k.device != q.device):
+            raise ValueError(f"{fn}: q {tuple(q.shape)} {q.dtype} on {q.device} and k {tuple(k.shape)} {k.dtype} on {k.device} must agree in "
+                             "batch, tokens, dtype and device")
+
+    def _check_append(self, q, k, v):
+        fn = "RotaryEmbedding.append"
+        self._check(fn, q, k)
+        if v.shape != k.shape or v.dtype is not k.dtype or v.device != k.device:
+            raise ValueError(f"{fn}: v {tuple(v.shape)} {v.dtype} must be like k {tuple(k.shape)} {k.dtype}")
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            raise ValueError(f"{fn}: not differentiable; rotate and append to the cache separately, or call it under torch.no_grad()")
+
+    @staticmethod
+    def _positions(fn, positions, B, S, device):
+        """(tensor or None, stride_b, stride_s, offset)."""
+        if positions is None:
+            return None, 0, 0, 0
+        if isinstance(positions, int):
+            return None, 0, 0, positions
+        if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{fn}: positions must be an int or an int32 / int64 tensor")
+        shape = tuple(positions.shape)
+        if shape not in ((S,), (1, S), (B, S)):
+            raise ValueError(f"{fn}: positions must be [{S}], [1, {S}] or [{B}, {S}], got {list(shape)}")
+        if positions.device != device:
+            raise ValueError(f"{fn}: positions are on {positions.device}, q on {device}")
+        st = positions.stride()
+        return positions, (st[0] if len(shape) == 2 and shape[0] == B and B > 1 else 0), st[-1], 0
+
+    def _launch(self, fn, B, S, dtype, device, tensors, positions, inverse) -> None:
+        """``tensors``: up to three ``(input, output or (address, strides))``; the third is copied."""
+        pos, psb, pss, off = self._positions(fn, positions, B, S, device)
+        a = RotaryArgs(dtype=dtype_code(dtype), B=B, S=S, D=self.head_dim, rotary_dim=self.rotary_dim,
+                       layout=1 if self.layout == "interleaved" else 0, inverse=1 if inverse else 0,
+                       positions=None if pos is None else pos.data_ptr(), pos_bytes=8 if pos is None else pos.element_size(),
+                       factor=self.attention_factor, pos_stride_b=psb, pos_stride_s=pss, pos_offset=off, turns=self._turns_on(device))
+        xs, ys = a.x_stride, a.y_stride
+        for i, (x, y) in enumerate(tensors):
+            a.x[i] = x.data_ptr()
+            a.heads[i] = x.shape[1]
+            xs[3 * i], xs[3 * i + 1], xs[3 * i + 2], _ = x.stride()
+            if isinstance(y, torch.Tensor):
+                a.y[i] = y.data_ptr()
+                ys[3 * i], ys[3 * i + 1], ys[3 * i + 2], _ = y.stride()
+            else:
+                a.y[i], (ys[3 * i], ys[3 * i + 1], ys[3 * i + 2], _) = y
+        with _lib.on_device(device):
+            check(lib().vq_rotary(a, stream_ptr(device)), fn)
+
+    # -- calls ---------------------------------------------------------------------------
+    def __call__(self, q: torch.Tensor, k: torch.Tensor | None = None, positions=None, *, inverse: bool = False):
+        fn = "RotaryEmbedding"
+        self._check(fn, q, k)
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+            out = _Rotate.apply(self, positions, inverse, q, k)
+        else:
+            out = self._rotate(fn, q, k, positions, inverse)
+        return out[0] if k is None else out
+
+    def _rotate(self, fn, q, k, positions, inverse):
+        require_cuda(q, f"{fn}: q")
+        pairs, out = [], []
+        for x in (q, k):
+            if x is None:
+                out.append(None)
+                continue
+            if x.stride(3) != 1:
+                x = x.contiguous()
+            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            pairs.append((x, y))
+            out.append(y)
+        self._launch(fn, q.shape[0], q.shape[2], q.dtype, q.device, pairs, positions, inverse)
+        return tuple(out)
+
+    def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_res: torch.Tensor, v_res: torch.Tensor, tok_offset: int,
+               positions=None) -> torch.Tensor:
+        """Turn ``q [B,H_q,S,D]`` and ``k [B,H_kv,S,D]`` in one launch, writing the turned keys and
+        ``v [B,H_kv,S,D]`` to rows ``[tok_offset, tok_offset + S)`` of ``k_res / v_res [B,H_kv,cap,D]``
+        (the exact window of a KIVI cache: the rotating form of ``kernels.kivi_append``); returns the
+        turned queries. The other rows stay as they are. Inputs must not share memory with
+        ``k_res`` / ``v_res``. Not differentiable."""
+        fn = "RotaryEmbedding.append"
+        self._check_append(q, k, v)
+        B, H, S, D = k.shape
+        for name, t in (("k_res", k_res), ("v_res", v_res)):
+            if t.ndim != 4 or t.shape[0] != B or t.shape[1] != H or t.shape[3] != D or t.dtype is not k.dtype or t.device != k.device:
+                raise ValueError(f"{fn}: {name} must be [{B}, {H}, rows, {D}] {k.dtype} on {k.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+            if t.stride(3) != 1 or t.stride(2) < D or 0 in t.stride()[:2]:
+                raise ValueError(f"{fn}: the channels of {name} must be contiguous and its rows apart, got strides {t.stride()}")
+            if tok_offset < 0 or tok_offset + S > t.shape[2]:
+                raise ValueError(f"{fn}: rows [{tok_offset}, {tok_offset + S}) exceed {name} ({t.shape[2]} rows)")
+        require_cuda(q, f"{fn}: q")
+        q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
+        if k_res.data_ptr() == v_res.data_ptr():
+            raise ValueError(f"{fn}: k_res and v_res must be different memory")
+        held = {k_res.untyped_storage().data_ptr(), v_res.untyped_storage().data_ptr()}
+        if any(t.untyped_storage().data_ptr() in held for t in (q, k, v)):
+            raise ValueError(f"{fn}: q, k and v must not share memory with k_res / v_res")
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        es = k.element_size()
+        rows = [(t.data_ptr() + tok_offset * t.stride(2) * es, t.stride()) for t in (k_res, v_res)]
+        self._launch(fn, B, S, q.dtype, q.device, ((q, out), (k, rows[0]), (v, rows[1])), positions, False)
+        return out
+
+
+class _Rotate(torch.autograd.Function):
+    """The turn as a differentiable operation: linear in q and k, its gradient is the inverse turn."""
+
+    @staticmethod
+    def forward(ctx, rope, positions, inverse, q, k):
+        ctx.rope, ctx.inverse = rope, inverse
+        ctx.set_materialize_grads(False)
+        ctx.tensor_positions = isinstance(positions, torch.Tensor)
+        if ctx.tensor_positions:
+            ctx.save_for_backward(positions)
+        else:
+            ctx.positions = positions
+        return rope._rotate("RotaryEmbedding", q, k, positions, inverse)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        positions = ctx.saved_tensors[0] if ctx.tensor_positions else ctx.positions
+        need_q, need_k = ctx.needs_input_grad[3], ctx.needs_input_grad[4]
+        gq, gk = gq if need_q else None, gk if need_k else None
+        if gq is not None and gk is not None:
+            gq, gk = _Rotate.apply(ctx.rope, positions, not ctx.inverse, gq, gk)
+        elif gq is not None:
+            gq = _Rotate.apply(ctx.rope, positions, not ctx.inverse, gq, None)[0]
+        elif gk is not None:
+            gk = _Rotate.apply(ctx.rope, positions, not ctx.inverse, gk, None)[0]
+        return None, None, None, gq, gk
+
+
+__all__ = ["RotaryEmbedding", "rotary_frequencies"]
