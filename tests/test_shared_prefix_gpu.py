@@ -143,7 +143,7 @@ CASES = [
 ]
 
 
-@pytest.mark.parametrize("variant", [0, 1])
+@pytest.mark.parametrize("variant", [0, 1, 2])
 @pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c))
 def test_against_64_bits(case, variant):
     B, Hq, Hk, S, D, bits, dtype, pq, pr, oq, orr = case
@@ -204,20 +204,21 @@ def test_a_later_token_outweighs_all_before_it():
     t["v_codes"], t["v_scale"], t["v_zero"] = kernels.kivi_quantize(v[:, :, :288], -1, 32, 4)
     t["k_res"], t["v_res"] = k[:, :, 288:].contiguous(), v[:, :, 288:].contiguous()
     pre = (KiviRows(**t), dense_of(t, 4, 288, D, 1, H))
-    for variant in (0, 1):
+    for variant in (1, 2):
         check(q.half(), pre, None, 0.5, variant=variant)
 
 
-@pytest.mark.parametrize("variant", [0, 1])
+@pytest.mark.parametrize("variant", [1, 2])
 def test_long_prefix_and_many_rows(variant):
     q = torch.randn(24, 8, 2, 128, device=DEV, generator=_gen(14)).to(BF)
     check(q, make_store(1, 2, 128, 4, 8192, 77, BF, 15), make_store(24, 2, 128, 4, 64, 40, BF, 16), 128**-0.5, variant=variant)
 
 
-@pytest.mark.parametrize("splits", [1, 2, 5, 64])
-def test_every_number_of_splits(splits):
+@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("splits", [1, 2, 5, 17, 64])
+def test_every_number_of_splits(splits, variant):
     q = torch.randn(12, 8, 1, 128, device=DEV, generator=_gen(17)).to(HF)
-    check(q, make_store(1, 2, 128, 4, 2080, 9, HF, 18), make_store(12, 2, 128, 4, 32, 1, HF, 19), 128**-0.5, n_splits=splits)
+    check(q, make_store(1, 2, 128, 4, 2080, 9, HF, 18), make_store(12, 2, 128, 4, 32, 1, HF, 19), 128**-0.5, n_splits=splits, variant=variant)
 
 
 def test_strided_queries_given_output_other_stream_and_repeat():

@@ -6,6 +6,7 @@
 
 #include "common.cuh"
 #include "kivi_attend.h"
+#include "shared_attend.h"
 
 namespace vq {
 
@@ -290,16 +291,19 @@ extern "C" int32_t vq_kivi_attend_splits(const vq_kivi_attend_args *args) {
 
 extern "C" int32_t vq_kivi_attend_status(void) {
     using namespace vq;
-    int flag = 0, flag2 = 0, flag3 = 0;
+    int flag = 0, flag2 = 0, flag3 = 0, flag4 = 0;
     int32_t rc = kivi_attend_mma_take_timeout(&flag);
     if (rc != VQ_OK) return rc;
     rc = coded_attend_take_timeout(&flag2);
     if (rc != VQ_OK) return rc;
     rc = peer_gather_take_timeout(&flag3);
     if (rc != VQ_OK) return rc;
+    rc = shared_prefix_tc5_take_timeout(&flag4);
+    if (rc != VQ_OK) return rc;
     if (flag3) return fail(VQ_ERR_TIMEOUT, "vq_peer_gather_wait: a peer's output rows did not arrive within the poll limit");
     if (flag) return fail(VQ_ERR_TIMEOUT, "vq_kivi_decode_attend: a bounded wait on a bulk-copy barrier gave up");
     if (flag2) return fail(VQ_ERR_TIMEOUT, "vq_rabitq_decode_attend: a bounded wait on a bulk-copy barrier gave up");
+    if (flag4) return fail(VQ_ERR_TIMEOUT, "vq_kivi_shared_attend: a bounded wait on an MMA or operand barrier gave up");
     return VQ_OK;
 }
 

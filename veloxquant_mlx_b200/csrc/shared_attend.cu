@@ -338,7 +338,7 @@ int32_t plan_of(const vq_shared_attend_args &a, const DeviceInfo &di, Plan *out)
     pl.prefix_tiles = (int)ceil_div(a.B * per_req, kRowTile);
     pl.own_tiles = (int)ceil_div(per_req, kRowTile);
     pl.no = go ? splits((int64_t)a.B * a.H_kv * pl.own_tiles, go) : 0;
-    pl.np = !gp ? 0 : a.n_splits > 0 ? std::min({a.n_splits, gp, 64}) : pl.tc5 ? shared_prefix_tc5_splits(a, di) : splits((int64_t)a.H_kv * pl.prefix_tiles, gp);
+    pl.np = !gp ? 0 : pl.tc5 ? shared_prefix_tc5_splits(a, di) : a.n_splits > 0 ? std::min({a.n_splits, gp, 64}) : splits((int64_t)a.H_kv * pl.prefix_tiles, gp);
     *out = pl;
     return VQ_OK;
 }
@@ -446,9 +446,3 @@ extern "C" int32_t vq_kivi_shared_attend(const vq_shared_attend_args *args, void
     if (a.dtype == VQ_F16) return a.D == 128 ? launch_all<128, __half>(a, pl, di, st) : launch_all<64, __half>(a, pl, di, st);
     return a.D == 128 ? launch_all<128, __nv_bfloat16>(a, pl, di, st) : launch_all<64, __nv_bfloat16>(a, pl, di, st);
 }
-
-namespace vq {
-const char *shared_prefix_tc5_supported(const vq_shared_attend_args &) { return "not built"; }
-int shared_prefix_tc5_splits(const vq_shared_attend_args &, const DeviceInfo &) { return 1; }
-int32_t shared_prefix_tc5_launch(const vq_shared_attend_args &, const SharedPartials &, int, const DeviceInfo &, cudaStream_t) { return VQ_ERR_SHAPE; }
-}  // namespace vq

@@ -28,7 +28,7 @@ template <int SB>
 struct Codes {
     static constexpr float kBase = SB == 8 ? 32768.f : 128.f;
     static constexpr int kPerWord = 32 / SB;
-    // Codes i of `w` whose index is a multiple of 8/SB ... shifted so that each sits alone in its byte.
+    // plane k of a word: its codes k, k + 8/SB, k + 2 * 8/SB, ..., each alone in its byte
     __device__ static __forceinline__ uint32_t plane(uint32_t w, int k) {
         if constexpr (SB == 8) return w;
         else return (w >> (SB * k)) & (SB == 4 ? 0x0f0f0f0fu : 0x03030303u);

@@ -1,0 +1,617 @@
+// The shared prefix on the fifth-generation tensor cores: all B * H_q/H_kv * S_q query rows of a kv
+// head against ONE copy of its packed keys and values.
+//
+// Per 128 query rows and 128 tokens: S = Q K^T (tcgen05.mma, float16 in, float32 in tensor memory),
+// P = 2^(S scale - m) (float16, back into tensor memory over S), O += P V (A operand from tensor
+// memory). Each CTA keeps two such streams in flight so that the softmax of one runs under the MMAs
+// of the other:
+//   more than 128 rows (TILES = 2): two row tiles share every decoded token tile;
+//   up to 128 rows     (TILES = 1): one row tile, the streams take token tiles in turn and leave two
+//                                   partial records.
+// Roles: warps 0-3 and 4-7 the softmax of stream 0 and 1 (a thread owns a row: no exchange between
+// lanes), warps 8-11 decode keys, 12-15 values, warp 16 issues the MMAs. Codes go from global memory to
+// registers one tile ahead, through one fused multiply-add and one rounding into 128-byte-swizzled
+// operand tiles, two stages each. Decoding once for 128 or 256 rows is what makes dense float16
+// operands affordable (the decode kernel for a few rows folds the scales into its queries instead).
+//
+// The reference maximum m of a row moves only when a tile exceeds it by more than 2^8 (weights up to
+// 256 are exact enough in float16 and cannot overflow its sums, which are float32): O in tensor
+// memory is then rescaled by the row's own thread. That S of step i + 1 is complete implies that P V
+// of step i is (MMAs of one thread complete in order), so no further wait is needed.
+//
+// Budget of a token tile with two row tiles at 4 bits, in SM clocks: MMAs 2048, exponentials 2048 (16 a
+// clock), instruction issue about 1900, HBM 1040.
+//
+// Every wait is bounded; a role that gives up raises a flag (reported by vq_kivi_attend_status), leaves its
+// loop, and the CTA still waits (bounded) for its MMAs and frees its tensor memory.
+#include <algorithm>
+
+#include "shared_attend.h"
+
+namespace vq {
+namespace {
+
+constexpr int kTile = 128;         // query rows of a stream = tensor-memory lanes; tokens of a tile
+constexpr int kGroup = 32;
+constexpr int kThreads = 17 * 32;
+constexpr uint32_t kSpin = 1u << 20;
+constexpr float kLazy = 8.f;       // log2 of how far a maximum may rise before O is rescaled
+
+__device__ int g_shared_timeout = 0;
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kSpin; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+
+// Shared-memory matrix descriptor with the 128-byte swizzle (tiles start on 1024-byte boundaries).
+// K-major: rows of 64 channels, 8-row groups `sbo` apart. MN-major: 64 channels of 8 tokens are one
+// 1024-byte block, token groups `sbo` apart, channel halves `lbo` apart.
+__device__ __forceinline__ uint64_t make_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    uint64_t d = 0;
+    d |= (uint64_t)((addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;
+    d |= (uint64_t)((sbo >> 4) & 0x3FFFu) << 32;
+    d |= 1ull << 46;  // descriptor version of this architecture
+    d |= 2ull << 61;  // 128-byte swizzle
+    return d;
+}
+// kind::f16, float16 operands, float32 accumulator, M = 128; B K-major or MN-major
+__device__ __forceinline__ constexpr uint32_t make_idesc(int N, bool b_mn_major) {
+    return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+                 "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+                 "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// The loaded values are threaded through the wait so that no use of them is scheduled ahead of it.
+__device__ __forceinline__ void tmem_ld_wait(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+                   "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]),
+                   "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
+                   "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+                 "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
+    uint32_t r[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+          "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+          "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+struct PrefixParams {
+    const void *q;
+    float scale_log2;
+    int B, H_q, H_kv, S_q, G;
+    vq_kivi_rows st;
+    SharedPartials parts;
+    int splits;       // CTAs along the tokens
+    int row_blocks;   // CTAs along the query rows of a kv head
+    int tiles_packed, tiles;
+};
+
+template <int D>
+struct Layout {
+    static constexpr int HALVES = D / 64;                     // 64-channel (128-byte) halves of a tile
+    static constexpr int HALF = kTile * 128;                  // bytes of one half
+    static constexpr int TILE = HALVES * HALF;
+    static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE;   // two Q tiles, two stages of K and V
+    static constexpr int BARS = 6 * TILE;
+    // padded past half an SM's shared memory: one CTA an SM, as it takes all of tensor memory
+    static constexpr int BYTES = BARS + 256 > 120 * 1024 ? BARS + 256 : 120 * 1024;
+    // 16-byte chunk `c` (0 .. D/8) of row `r`
+    __device__ static __forceinline__ uint32_t at(int r, int c) { return (uint32_t)((c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
+};
+
+enum { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPReady = 10, kODone = 12, kDrain = 14, kBars = 15 };
+
+__device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
+
+// 8 neighbouring codes of a row (SB bytes) as 8 halves
+template <int SB>
+__device__ __forceinline__ uint4 decode8(const uint32_t (&w)[SB == 8 ? 2 : 1], const float (&sc)[8], const float (&ze)[8]) {
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        constexpr int per = Codes<SB>::kPerWord;
+        r[i] = pack_f16(fmaf(Codes<SB>::get(w[2 * i / per], 2 * i % per), sc[2 * i], ze[2 * i]),
+                        fmaf(Codes<SB>::get(w[(2 * i + 1) / per], (2 * i + 1) % per), sc[2 * i + 1], ze[2 * i + 1]));
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <int D, int SB, typename T, int TILES>
+__global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __grid_constant__ PrefixParams p) {
+    using L = Layout<D>;
+    constexpr int CHUNKS = D / 8;      // 8-channel chunks of a row
+    constexpr int RB = D * SB / 8;     // bytes of a packed row
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BARS);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::BARS + 8 * kBars);
+    const uint32_t bar0 = smem_u32(bars);
+    auto bar = [&](int i) { return bar0 + 8u * i; };
+
+    int blk = blockIdx.x;
+    const int split = blk % p.splits; blk /= p.splits;
+    const int rb = blk % p.row_blocks;
+    const int hk = blk / p.row_blocks;
+    const int per_req = p.G * p.S_q, n_rows = p.B * per_req;
+    const int row0 = rb * kTile * TILES;
+    const int t_lo = (int)((int64_t)p.tiles * split / p.splits), t_hi = (int)((int64_t)p.tiles * (split + 1) / p.splits);
+    const int n_tiles = t_hi - t_lo;
+    const int n_steps = TILES == 2 ? 2 * n_tiles : n_tiles;
+    const vq_kivi_rows &st = p.st;
+
+    auto out_row = [&](int r) {  // output row (= row of q) of this kv head's query row r
+        const int b = r / per_req;
+        return ((int64_t)b * p.H_q + (int64_t)hk * p.G) * p.S_q + (r - b * per_req);
+    };
+
+    if ((smem_u32(smem) & 1023u) != 0) {  // the swizzle assumes it; never seen
+        if (tid == 0) atomicExch(&g_shared_timeout, 2);
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < kBars; ++i) {
+            const bool by_warps = i < kKEmpty || (i >= kVFull && i < kVEmpty) || (i >= kPReady && i < kODone);
+            mbar_init(bar(i), by_warps ? 4 : 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 16) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // the query tiles, as halves; rows behind the last are zero
+    for (int i = tid; i < TILES * kTile * CHUNKS; i += kThreads) {
+        const int r = i / CHUNKS, c = i % CHUNKS;
+        uint4 v = zero4();
+        if (row0 + r < n_rows) {
+            v = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(p.q) + out_row(row0 + r) * D) + c);
+            v = make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w));
+        }
+        *reinterpret_cast<uint4 *>(smem + L::Q + (r / kTile) * L::TILE + L::at(r % kTile, c)) = v;
+    }
+    fence_async_smem();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem_s[2] = {tmem, tmem + 128}, tmem_o[2] = {tmem + 256, tmem + 384};
+    bool gave_up = false;
+    auto wait = [&](int b, uint32_t parity) {  // by whole warps: all lanes go on or none
+        if (!gave_up) gave_up = !__all_sync(0xffffffffu, mbar_wait(bar(b), parity));
+        return !gave_up;
+    };
+    auto wait_one = [&](int b, uint32_t parity) {  // by the one thread that issues the MMAs
+        if (!gave_up && !mbar_wait(bar(b), parity)) gave_up = true;
+        return !gave_up;
+    };
+
+    if (warp < 8) {
+        // ---- softmax: thread = row -----------------------------------------------------------------
+        const int s = warp >> 2;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem_s[s] + lane_base, to = tmem_o[s] + lane_base;
+        const int n_mine = TILES == 2 ? n_tiles : (n_tiles - s + 1) / 2;
+        float m = -INFINITY, l = 0.f;  // reference maximum (times scale, base 2) and the weights' sum
+        for (int i = 0; i < n_mine; ++i) {
+            const int t = t_lo + (TILES == 2 ? i : 2 * i + s);
+            const int nv = t < p.tiles_packed ? min(kTile, st.n_quant - t * kTile) : min(kTile, st.n_res - (t - p.tiles_packed) * kTile);
+            if (!wait(kSFull + s, i & 1)) break;
+            fence_after();
+            float mx = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float v[32];
+                tmem_ld32(ts + 32 * c, v);
+                tmem_ld_wait(v);
+                if (nv < 32 * (c + 1)) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[k] = 32 * c + k < nv ? v[k] : -INFINITY;
+                }
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) mx = max3(mx, v[k], v[k + 1]);
+            }
+            mx *= p.scale_log2;
+            const bool raise = mx > m + kLazy || (m == -INFINITY && mx != -INFINITY);
+            if (__any_sync(0xffffffffu, raise)) {
+                const float mn = raise ? mx : m;
+                const float f = m == -INFINITY ? 0.f : ex2(m - mn);
+                m = mn;
+                l *= f;
+                if (i > 0) {
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        float v[32];
+                        tmem_ld32(to + 32 * c, v);
+                        tmem_ld_wait(v);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] *= f;
+                        tmem_st32(to + 32 * c, v);
+                    }
+                }
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+            float sum[4] = {};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float v[32];
+                tmem_ld32(ts + 32 * c, v);
+                tmem_ld_wait(v);
+                uint32_t r[16];
+#pragma unroll
+                for (int k = 0; k < 32; ++k) v[k] = ex2(fmaf(v[k], p.scale_log2, -base));
+                if (nv < 32 * (c + 1)) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[k] = 32 * c + k < nv ? v[k] : 0.f;
+                }
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    sum[k & 3] += v[2 * k] + v[2 * k + 1];
+                    r[k] = pack_f16(v[2 * k], v[2 * k + 1]);
+                }
+                tmem_st16(ts + 16 * c, r);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(kPReady + s));
+        }
+        if (n_mine > 0) wait(kODone + s, 0);
+        fence_after();
+        const int r = row0 + (TILES == 2 ? s * kTile : 0) + (warp & 3) * 32 + lane;
+        const bool live = r < n_rows;
+        const int64_t rec = live ? out_row(r) * p.parts.n_splits + (TILES == 2 ? split : 2 * split + s) : 0;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+            float v[32];
+            tmem_ld32(to + 32 * c, v);
+            tmem_ld_wait(v);
+            if (live) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 4)
+                    *reinterpret_cast<float4 *>(p.parts.o + rec * D + 32 * c + k) =
+                        n_mine > 0 ? make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        }
+        if (live) *reinterpret_cast<float2 *>(p.parts.ml + rec * 2) = make_float2(m, l);
+    } else if (warp < 12) {
+        // ---- keys: warp w decodes the w-th 32-token group of a tile -----------------------------------
+        // lane = (token parity, chunk of 8 channels): the group's scales and zeros of 8 channels stay in registers
+        constexpr int TPL = 32 / CHUNKS;          // tokens a warp covers at once: 2 (D = 128) or 4
+        constexpr int N = kGroup / TPL;           // tokens a lane decodes
+        constexpr int W = SB == 8 ? 2 : 1;
+        const int w = warp - 8, chunk = lane % CHUNKS, sub = lane / CHUNKS;
+        const uint8_t *codes = st.k_codes + hk * st.k_codes_stride_bh;
+        const float *ks = st.k_scale + hk * st.k_param_stride_bh, *kz = st.k_zero + hk * st.k_param_stride_bh;
+        const T *exact = reinterpret_cast<const T *>(st.k_res) + hk * st.res_stride_bh;
+        uint32_t next[N][W];
+        float4 ns[2], nz[2];
+        auto fetch = [&](int t) {
+            const int grp = t * (kTile / kGroup) + w;
+            if (t >= p.tiles_packed || grp * kGroup >= st.n_quant) return;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const uint8_t *src = codes + (int64_t)(grp * kGroup + TPL * i + sub) * RB + chunk * SB;
+                if constexpr (SB == 8) {
+                    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(src));
+                    next[i][0] = v.x; next[i][1] = v.y;
+                } else if constexpr (SB == 4) next[i][0] = __ldg(reinterpret_cast<const uint32_t *>(src));
+                else next[i][0] = __ldg(reinterpret_cast<const uint16_t *>(src));
+            }
+            const float4 *s4 = reinterpret_cast<const float4 *>(ks + (int64_t)grp * D + 8 * chunk);
+            const float4 *z4 = reinterpret_cast<const float4 *>(kz + (int64_t)grp * D + 8 * chunk);
+            ns[0] = __ldg(s4); ns[1] = __ldg(s4 + 1);
+            nz[0] = __ldg(z4); nz[1] = __ldg(z4 + 1);
+        };
+        if (n_tiles > 0) fetch(t_lo);
+        for (int i = 0; i < n_tiles; ++i) {
+            const int t = t_lo + i, stage = i & 1;
+            uint8_t *dst = smem + L::K + stage * L::TILE;
+            const bool packed = t < p.tiles_packed;
+            if (packed) {
+                const bool some = t * kTile + w * kGroup < st.n_quant;
+                uint32_t cur[N][W];
+                const float sc[8] = {ns[0].x, ns[0].y, ns[0].z, ns[0].w, ns[1].x, ns[1].y, ns[1].z, ns[1].w};
+                const float zz[8] = {nz[0].x, nz[0].y, nz[0].z, nz[0].w, nz[1].x, nz[1].y, nz[1].z, nz[1].w};
+                float ze[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) ze[k] = fmaf(-Codes<SB>::kBase, sc[k], zz[k]);
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+#pragma unroll
+                    for (int j = 0; j < W; ++j) cur[k][j] = next[k][j];
+                if (i + 1 < n_tiles) fetch(t + 1);
+                if (i >= 2 && !wait(kKEmpty + stage, ((i >> 1) - 1) & 1)) break;
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+                    *reinterpret_cast<uint4 *>(dst + L::at(w * kGroup + TPL * k + sub, chunk)) = some ? decode8<SB>(cur[k], sc, ze) : zero4();
+            } else {
+                if (i >= 2 && !wait(kKEmpty + stage, ((i >> 1) - 1) & 1)) break;
+                const int r0 = (t - p.tiles_packed) * kTile + w * kGroup;
+#pragma unroll 4
+                for (int k = 0; k < N; ++k) {
+                    const int row = r0 + TPL * k + sub;
+                    uint4 v = zero4();
+                    if (row < st.n_res) {
+                        v = __ldg(reinterpret_cast<const uint4 *>(exact + (int64_t)row * D) + chunk);
+                        v = make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w));
+                    }
+                    *reinterpret_cast<uint4 *>(dst + L::at(w * kGroup + TPL * k + sub, chunk)) = v;
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(kKFull + stage));
+        }
+    } else if (warp < 16) {
+        // ---- values: a thread decodes one 32-channel group (one scale, one zero) of a token ------------
+        constexpr int GV = D / kGroup;            // value groups of a token = threads of a token
+        constexpr int TPI = 128 / GV;             // tokens the four warps cover at once
+        constexpr int N = kTile / TPI;            // tokens a thread decodes
+        constexpr int W = SB;                     // words of 32 codes
+        const int vt = tid - 12 * 32, grp = vt % GV, tok = vt / GV;
+        const uint8_t *codes = st.v_codes + hk * st.v_codes_stride_bh;
+        const float *vs = st.v_scale + hk * st.v_param_stride_bh, *vz = st.v_zero + hk * st.v_param_stride_bh;
+        const T *exact = reinterpret_cast<const T *>(st.v_res) + hk * st.res_stride_bh;
+        uint32_t next[N][W];
+        float ns[N], nz[N];
+        auto fetch = [&](int t) {
+            if (t >= p.tiles_packed) return;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int64_t slot = (int64_t)t * kTile + i * TPI + tok;
+                if (slot >= st.n_quant) break;
+                const uint8_t *src = codes + slot * RB + grp * (4 * SB);
+                if constexpr (W == 2) {
+                    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(src));
+                    next[i][0] = v.x; next[i][1] = v.y;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < W; j += 4) {
+                        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src) + j / 4);
+                        next[i][j] = v.x; next[i][j + 1] = v.y; next[i][j + 2] = v.z; next[i][j + 3] = v.w;
+                    }
+                }
+                ns[i] = __ldg(vs + slot * GV + grp);
+                nz[i] = __ldg(vz + slot * GV + grp);
+            }
+        };
+        if (n_tiles > 0) fetch(t_lo);
+        for (int i = 0; i < n_tiles; ++i) {
+            const int t = t_lo + i, stage = i & 1;
+            uint8_t *dst = smem + L::V + stage * L::TILE;
+            if (t < p.tiles_packed) {
+                uint32_t cur[N][W];
+                float sc[N], ze[N];
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    sc[k] = ns[k];
+                    ze[k] = fmaf(-Codes<SB>::kBase, ns[k], nz[k]);
+#pragma unroll
+                    for (int j = 0; j < W; ++j) cur[k][j] = next[k][j];
+                }
+                if (i + 1 < n_tiles) fetch(t + 1);
+                if (i >= 2 && !wait(kVEmpty + stage, ((i >> 1) - 1) & 1)) break;
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const int row = k * TPI + tok;
+                    const bool some = t * kTile + row < st.n_quant;
+                    const float s8[8] = {sc[k], sc[k], sc[k], sc[k], sc[k], sc[k], sc[k], sc[k]};
+                    const float z8[8] = {ze[k], ze[k], ze[k], ze[k], ze[k], ze[k], ze[k], ze[k]};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t wd[SB == 8 ? 2 : 1];
+                        if constexpr (SB == 8) { wd[0] = cur[k][2 * j]; wd[1] = cur[k][2 * j + 1]; }
+                        else if constexpr (SB == 4) wd[0] = cur[k][j];
+                        else wd[0] = cur[k][j / 2] >> (16 * (j & 1));
+                        *reinterpret_cast<uint4 *>(dst + L::at(row, 4 * grp + j)) = some ? decode8<SB>(wd, s8, z8) : zero4();
+                    }
+                }
+            } else {
+                if (i >= 2 && !wait(kVEmpty + stage, ((i >> 1) - 1) & 1)) break;
+                const int r0 = (t - p.tiles_packed) * kTile;
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const int row = k * TPI + tok;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint4 v = zero4();
+                        if (r0 + row < st.n_res) {
+                            v = __ldg(reinterpret_cast<const uint4 *>(exact + (int64_t)(r0 + row) * D) + 4 * grp + j);
+                            v = make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w));
+                        }
+                        *reinterpret_cast<uint4 *>(dst + L::at(row, 4 * grp + j)) = v;
+                    }
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(kVFull + stage));
+        }
+    } else if (lane == 0) {
+        // ---- the MMAs, all by one thread, in order ------------------------------------------------------
+        const uint32_t sq = smem_u32(smem + L::Q), sk = smem_u32(smem + L::K), sv = smem_u32(smem + L::V);
+        auto qk = [&](int j) {
+            const int s = j & 1, t = TILES == 2 ? j >> 1 : j, stage = t & 1;
+            if ((TILES == 1 || s == 0) && !wait_one(kKFull + stage, (t >> 1) & 1)) return;
+            fence_after();
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = (uint32_t)((k >> 2) * L::HALF + (k & 3) * 32);
+                mma_ss(tmem_s[s], make_desc(sq + (TILES == 2 ? s * L::TILE : 0) + off, 16, 1024), make_desc(sk + stage * L::TILE + off, 16, 1024),
+                       make_idesc(kTile, false), k > 0);
+            }
+            mma_commit(bar(kSFull + s));
+            if (TILES == 1 || s == 1) mma_commit(bar(kKEmpty + stage));
+        };
+        auto pv = [&](int j) {
+            const int s = j & 1, t = TILES == 2 ? j >> 1 : j, stage = t & 1;
+            if ((TILES == 1 || s == 0) && !wait_one(kVFull + stage, (t >> 1) & 1)) return;
+            if (!wait_one(kPReady + s, (j >> 1) & 1)) return;
+            fence_after();
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k)
+                mma_ts(tmem_o[s], tmem_s[s] + 8 * k, make_desc(sv + stage * L::TILE + k * 2048, L::HALF, 1024), make_idesc(D, true), j >= 2 || k > 0);
+            if (TILES == 1 || s == 1) mma_commit(bar(kVEmpty + stage));
+            if (j + 2 >= n_steps) mma_commit(bar(kODone + s));
+        };
+        if (n_steps > 0) qk(0);
+        if (n_steps > 1) qk(1);
+        for (int j = 0; j < n_steps && !gave_up; ++j) {
+            pv(j);
+            if (j + 2 < n_steps && !gave_up) qk(j + 2);
+        }
+        if (gave_up) {  // MMAs in flight still use shared and tensor memory
+            mma_commit(bar(kDrain));
+            mbar_wait(bar(kDrain), 0);
+        }
+    }
+    if (gave_up) atomicExch(&g_shared_timeout, 1);
+    fence_before();
+    __syncthreads();
+    if (warp == 16) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+int64_t rows_of(const vq_shared_attend_args &a) { return (int64_t)a.B * (a.H_q / a.H_kv) * a.S_q; }
+int tiles_of(const vq_shared_attend_args &a) { return (int)(ceil_div(a.prefix.n_quant, kTile) + ceil_div(a.prefix.n_res, kTile)); }
+int row_tiles(const vq_shared_attend_args &a) { return rows_of(a) > kTile ? 2 : 1; }
+
+template <int D, int SB, typename T, int TILES>
+int32_t launch(const PrefixParams &p, unsigned blocks, cudaStream_t st) {
+    VQ_CHECK_CUDA(cudaFuncSetAttribute(shared_prefix_tc5_kernel<D, SB, T, TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::BYTES));
+    shared_prefix_tc5_kernel<D, SB, T, TILES><<<blocks, kThreads, Layout<D>::BYTES, st>>>(p);
+    VQ_CHECK_LAUNCH("shared_prefix_tc5_kernel");
+    return VQ_OK;
+}
+template <int D, int SB, typename T>
+int32_t launch_rows(const PrefixParams &p, int tiles, unsigned blocks, cudaStream_t st) {
+    return tiles == 2 ? launch<D, SB, T, 2>(p, blocks, st) : launch<D, SB, T, 1>(p, blocks, st);
+}
+template <int D, typename T>
+int32_t launch_bits(int sb, const PrefixParams &p, int tiles, unsigned blocks, cudaStream_t st) {
+    if (sb == 2) return launch_rows<D, 2, T>(p, tiles, blocks, st);
+    if (sb == 4) return launch_rows<D, 4, T>(p, tiles, blocks, st);
+    return launch_rows<D, 8, T>(p, tiles, blocks, st);
+}
+
+}  // namespace
+
+const char *shared_prefix_tc5_supported(const vq_shared_attend_args &a) {
+    if (!(a.scale >= 0.f)) return "the scale must not be negative";
+    if (a.prefix.n_quant + a.prefix.n_res == 0) return "the prefix is empty";
+    // up to two warp tiles of 16 rows decode a token no more often than this kernel's setup costs
+    if (a.variant != 2 && (rows_of(a) <= 32 || tiles_of(a) < 4)) return "few query rows or tokens";
+    return nullptr;
+}
+
+// Partial records of the prefix: one per split, two where the streams share a row tile.
+int shared_prefix_tc5_splits(const vq_shared_attend_args &a, const DeviceInfo &di) {
+    const int tiles = tiles_of(a), rt = row_tiles(a);
+    const int64_t units = (int64_t)a.H_kv * ceil_div(rows_of(a), kTile * rt);
+    int best = 1;
+    if (a.n_splits > 0) {
+        best = std::min({a.n_splits, tiles, 32});
+    } else {
+        // The time of a split count, in token tiles: waves of CTAs (one an SM) times the longest CTA (its
+        // tiles and a fixed part for setup and epilogue), plus the merge's reading of the records.
+        double cheapest = 1e30;
+        for (int s = 1; s <= std::min(tiles, 32); ++s) {
+            const double waves = (double)ceil_div(units * s, di.sm_count);
+            const double t = waves * ((double)ceil_div(tiles, s) + 3.0) + 0.02 * s * (double)ceil_div(units * rt * s, di.sm_count);
+            if (t < cheapest) { cheapest = t; best = s; }
+        }
+    }
+    return rt == 1 ? 2 * best : best;
+}
+
+int32_t shared_prefix_tc5_launch(const vq_shared_attend_args &a, const SharedPartials &parts, int np, const DeviceInfo &di, cudaStream_t st) {
+    (void)di;
+    const int rt = row_tiles(a);
+    PrefixParams p = {};
+    p.q = a.q;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.B = a.B; p.H_q = a.H_q; p.H_kv = a.H_kv; p.S_q = a.S_q; p.G = a.H_q / a.H_kv;
+    p.st = a.prefix;
+    p.parts = parts;
+    p.splits = rt == 1 ? np / 2 : np;
+    p.row_blocks = (int)ceil_div(rows_of(a), kTile * rt);
+    p.tiles_packed = (int)ceil_div(a.prefix.n_quant, kTile);
+    p.tiles = tiles_of(a);
+    const int64_t blocks = (int64_t)p.splits * p.row_blocks * a.H_kv;
+    VQ_REQUIRE(blocks < (1ll << 31), VQ_ERR_SHAPE, "vq_kivi_shared_attend: too many query rows for one launch");
+    const unsigned nb = (unsigned)blocks;
+    if (a.dtype == VQ_F16) return a.D == 128 ? launch_bits<128, __half>(a.store_bits, p, rt, nb, st) : launch_bits<64, __half>(a.store_bits, p, rt, nb, st);
+    return a.D == 128 ? launch_bits<128, __nv_bfloat16>(a.store_bits, p, rt, nb, st) : launch_bits<64, __nv_bfloat16>(a.store_bits, p, rt, nb, st);
+}
+
+int32_t shared_prefix_tc5_take_timeout(int *flag) {
+    VQ_CHECK_CUDA(cudaDeviceSynchronize());
+    const int zero = 0;
+    VQ_CHECK_CUDA(cudaMemcpyFromSymbol(flag, g_shared_timeout, sizeof(int)));
+    VQ_CHECK_CUDA(cudaMemcpyToSymbol(g_shared_timeout, &zero, sizeof(int)));
+    return VQ_OK;
+}
+
+}  // namespace vq
