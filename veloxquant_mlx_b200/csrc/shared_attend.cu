@@ -8,6 +8,7 @@
 // The prefix is read once for all B * H_q/H_kv * S_q query rows of a kv head (from 33 rows on by the
 // tcgen05 kernel of shared_prefix_tc5.cu), the own tokens once per request.
 #include <algorithm>
+#include <type_traits>
 
 #include "kivi_attend.h"
 #include "shared_attend.h"
@@ -284,32 +285,66 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
     }
 }
 
-// One warp joins the records of one output row. Bound by latency: a few KB a row.
+// Joins the records of an output row: `ways` warps (1 or 4) take its records in turn, each lane D/32
+// channels; every warp has all of the row's (m, l) in its lanes. Bound by latency (a few KB a row, from
+// L2), so eight records are requested at a time.
+constexpr int kMaxRecords = 128;  // 64 splits of either part
+
 template <int D, typename T>
-__global__ void __launch_bounds__(128) shared_attend_merge_kernel(const SharedPartials parts, int64_t rows, T *__restrict__ out, float *__restrict__ lse) {
-    constexpr int C = D / 32;  // channels a lane
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= rows) return;
+__global__ void __launch_bounds__(128) shared_attend_merge_kernel(const SharedPartials parts, int64_t rows, int ways, T *__restrict__ out, float *__restrict__ lse) {
+    constexpr int C = D / 32;
+    using V = typename std::conditional<C == 4, float4, float2>::type;
+    __shared__ float sh[4][D];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int part = warp % ways;
+    const int64_t row = (int64_t)blockIdx.x * (4 / ways) + warp / ways;
     const int n = parts.n_splits;
-    const float *ml = parts.ml + row * n * 2;
-    float mm = -INFINITY;
-    for (int j = lane; j < n; j += 32) mm = fmaxf(mm, ml[2 * j]);
-    mm = warp_max(mm);
-    const float bs = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f, acc[C] = {};
-    const float *po = parts.o + row * n * D + lane * C;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-        const float2 r = *reinterpret_cast<const float2 *>(ml + 2 * j);
-        const float f = ex2(r.x - bs);
-        ll = fmaf(r.y, f, ll);
+    float ll = 0.f, mm = -INFINITY, acc[C] = {};
+    if (row < rows) {
+        const float2 *ml = reinterpret_cast<const float2 *>(parts.ml) + row * n;
+        float2 r[kMaxRecords / 32];
 #pragma unroll
-        for (int c = 0; c < C; ++c) acc[c] = fmaf(po[(int64_t)j * D + c], f, acc[c]);
+        for (int i = 0; i < kMaxRecords / 32; ++i) {
+            r[i] = 32 * i + lane < n ? ml[32 * i + lane] : make_float2(-INFINITY, 0.f);
+            mm = fmaxf(mm, r[i].x);
+        }
+        mm = warp_max(mm);
+        const float bs = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+        for (int i = 0; i < kMaxRecords / 32; ++i) {
+            r[i].x = ex2(r[i].x - bs);  // the record's weight
+            ll = fmaf(r[i].y, r[i].x, ll);
+        }
+        ll = warp_sum(ll);
+        const V *po = reinterpret_cast<const V *>(parts.o + row * n * D) + lane;
+#pragma unroll
+        for (int i = 0; i < kMaxRecords / 32; ++i) {
+            const int last = min(32, n - 32 * i);
+#pragma unroll 8
+            for (int j = part; j < last; j += ways) {
+                const V v = po[(int64_t)(32 * i + j) * 32];
+                const float f = __shfl_sync(0xffffffffu, r[i].x, j);
+                const float *e = reinterpret_cast<const float *>(&v);
+#pragma unroll
+                for (int c = 0; c < C; ++c) acc[c] = fmaf(e[c], f, acc[c]);
+            }
+        }
     }
-    const float inv = ll > 0.f ? 1.f / ll : ll == 0.f ? 0.f : ll;  // nothing seen: zeros; NaN stays
+    if (ways > 1) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) out[row * D + lane * C + c] = from_f32<T>(acc[c] * inv);
+        for (int c = 0; c < C; ++c) sh[warp][lane * C + c] = acc[c];
+        __syncthreads();
+        if (warp != 0) return;
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] = (sh[0][lane * C + c] + sh[1][lane * C + c]) + (sh[2][lane * C + c] + sh[3][lane * C + c]);
+    }
+    if (row >= rows) return;
+    const float inv = ll > 0.f ? 1.f / ll : ll == 0.f ? 0.f : ll;  // nothing seen: zeros; NaN stays
+    alignas(8) T res[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) res[c] = from_f32<T>(acc[c] * inv);
+    using O = typename std::conditional<C == 4, uint2, uint32_t>::type;
+    reinterpret_cast<O *>(out + row * D)[lane] = *reinterpret_cast<const O *>(res);
     if (lse && lane == 0) lse[row] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
 }
 
@@ -408,7 +443,8 @@ int32_t launch_all(const vq_shared_attend_args &a, const Plan &pl, const DeviceI
         else shared_attend_rows_kernel<D, 8, T><<<(unsigned)blocks, kWarps * 32, 0, st>>>(p);
         VQ_CHECK_LAUNCH("shared_attend_rows_kernel");
     }
-    shared_attend_merge_kernel<D, T><<<(unsigned)ceil_div(pl.rows, 4), 128, 0, st>>>(p.parts, pl.rows, (T *)a.out, a.lse);
+    const int ways = p.parts.n_splits > 8 ? 4 : 1;
+    shared_attend_merge_kernel<D, T><<<(unsigned)ceil_div(pl.rows * ways, 4), 128, 0, st>>>(p.parts, pl.rows, ways, (T *)a.out, a.lse);
     VQ_CHECK_LAUNCH("shared_attend_merge_kernel");
     return VQ_OK;
 }

@@ -105,6 +105,16 @@ __device__ __forceinline__ void tmem_ld_wait(float (&v)[32]) {
                  :
                  : "memory");
 }
+// The same for an array loaded before a tmem_ld_wait of another (both statements keep their order).
+__device__ __forceinline__ void tmem_pin(float (&v)[32]) {
+    asm volatile(""
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+                   "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]),
+                   "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
+                   "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
@@ -131,6 +141,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
+}
+
+// Columns from `n` on (of 64 in two arrays) become `x`.
+__device__ __forceinline__ void drop_from(float (&v)[32], float (&w)[32], int n, float x) {
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+        v[k] = k < n ? v[k] : x;
+        w[k] = 32 + k < n ? w[k] : x;
+    }
 }
 
 struct PrefixParams {
@@ -233,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
     __syncthreads();
     fence_after();
     const uint32_t tmem = *tmem_slot;
-    const uint32_t tmem_s[2] = {tmem, tmem + 128}, tmem_o[2] = {tmem + 256, tmem + 384};
+    // scores (and the weights over them) of stream s: columns 128 s; its output: 256 + 128 s
     bool gave_up = false;
     auto wait = [&](int b, uint32_t parity) {  // by whole warps: all lanes go on or none
         if (!gave_up) gave_up = !__all_sync(0xffffffffu, mbar_wait(bar(b), parity));
@@ -248,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
         // ---- softmax: thread = row -----------------------------------------------------------------
         const int s = warp >> 2;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem_s[s] + lane_base, to = tmem_o[s] + lane_base;
+        const uint32_t ts = tmem + 128 * s + lane_base, to = ts + 256;
         const int n_mine = TILES == 2 ? n_tiles : (n_tiles - s + 1) / 2;
         float m = -INFINITY, l = 0.f;  // reference maximum (times scale, base 2) and the weights' sum
         for (int i = 0; i < n_mine; ++i) {
@@ -257,17 +276,21 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
             if (!wait(kSFull + s, i & 1)) break;
             fence_after();
             float mx = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float v[32];
-                tmem_ld32(ts + 32 * c, v);
+#pragma unroll 1
+            for (int c = 0; c < kTile; c += 64) {
+                float v[32], w[32];
+                tmem_ld32(ts + c, v);
+                tmem_ld32(ts + c + 32, w);
                 tmem_ld_wait(v);
-                if (nv < 32 * (c + 1)) {
+                tmem_pin(w);
+                if (nv < c + 64) drop_from(v, w, nv - c, -INFINITY);
+                float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] = 32 * c + k < nv ? v[k] : -INFINITY;
+                for (int k = 0; k < 32; k += 2) {
+                    m4[(k >> 1) & 1] = max3(m4[(k >> 1) & 1], v[k], v[k + 1]);
+                    m4[2 + ((k >> 1) & 1)] = max3(m4[2 + ((k >> 1) & 1)], w[k], w[k + 1]);
                 }
-#pragma unroll
-                for (int k = 0; k < 32; k += 2) mx = max3(mx, v[k], v[k + 1]);
+                mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
             }
             mx *= p.scale_log2;
             const bool raise = mx > m + kLazy || (m == -INFINITY && mx != -INFINITY);
@@ -277,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
                 m = mn;
                 l *= f;
                 if (i > 0) {
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < D / 32; ++c) {
                         float v[32];
                         tmem_ld32(to + 32 * c, v);
@@ -290,24 +313,31 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
             }
             const float base = m == -INFINITY ? 0.f : m;
             float sum[4] = {};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float v[32];
-                tmem_ld32(ts + 32 * c, v);
+#pragma unroll 1
+            for (int c = 0; c < kTile; c += 64) {
+                float v[32], w[32];
+                tmem_ld32(ts + c, v);
+                tmem_ld32(ts + c + 32, w);
                 tmem_ld_wait(v);
-                uint32_t r[16];
+                tmem_pin(w);
 #pragma unroll
                 for (int k = 0; k < 32; ++k) v[k] = ex2(fmaf(v[k], p.scale_log2, -base));
-                if (nv < 32 * (c + 1)) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] = 32 * c + k < nv ? v[k] : 0.f;
-                }
+                for (int k = 0; k < 32; ++k) w[k] = ex2(fmaf(w[k], p.scale_log2, -base));
+                if (nv < c + 64) drop_from(v, w, nv - c, 0.f);
+                uint32_t r[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
                     sum[k & 3] += v[2 * k] + v[2 * k + 1];
                     r[k] = pack_f16(v[2 * k], v[2 * k + 1]);
                 }
-                tmem_st16(ts + 16 * c, r);
+                tmem_st16(ts + c / 2, r);  // (over scores that have been read)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    sum[k & 3] += w[2 * k] + w[2 * k + 1];
+                    r[k] = pack_f16(w[2 * k], w[2 * k + 1]);
+                }
+                tmem_st16(ts + c / 2 + 16, r);
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -320,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
         const int r = row0 + (TILES == 2 ? s * kTile : 0) + (warp & 3) * 32 + lane;
         const bool live = r < n_rows;
         const int64_t rec = live ? out_row(r) * p.parts.n_splits + (TILES == 2 ? split : 2 * split + s) : 0;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
             float v[32];
             tmem_ld32(to + 32 * c, v);
@@ -343,51 +373,49 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
         const uint8_t *codes = st.k_codes + hk * st.k_codes_stride_bh;
         const float *ks = st.k_scale + hk * st.k_param_stride_bh, *kz = st.k_zero + hk * st.k_param_stride_bh;
         const T *exact = reinterpret_cast<const T *>(st.k_res) + hk * st.res_stride_bh;
-        uint32_t next[N][W];
-        float4 ns[2], nz[2];
-        auto fetch = [&](int t) {
-            const int grp = t * (kTile / kGroup) + w;
-            if (t >= p.tiles_packed || grp * kGroup >= st.n_quant) return;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const uint8_t *src = codes + (int64_t)(grp * kGroup + TPL * i + sub) * RB + chunk * SB;
-                if constexpr (SB == 8) {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(src));
-                    next[i][0] = v.x; next[i][1] = v.y;
-                } else if constexpr (SB == 4) next[i][0] = __ldg(reinterpret_cast<const uint32_t *>(src));
-                else next[i][0] = __ldg(reinterpret_cast<const uint16_t *>(src));
-            }
-            const float4 *s4 = reinterpret_cast<const float4 *>(ks + (int64_t)grp * D + 8 * chunk);
-            const float4 *z4 = reinterpret_cast<const float4 *>(kz + (int64_t)grp * D + 8 * chunk);
+        uint32_t cur[N][W];   // codes of the tile to decode; each is replaced by the next tile's once it is used
+        float4 ns[2], nz[2];  // its scales and zeros
+        auto here = [&](int t) { return t < min(t_hi, p.tiles_packed) && t * kTile + w * kGroup < st.n_quant; };
+        auto fetch_codes = [&](int t, int i) {
+            const uint8_t *src = codes + ((int64_t)t * kTile + w * kGroup + TPL * i + sub) * RB + chunk * SB;
+            if constexpr (SB == 8) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(src));
+                cur[i][0] = v.x; cur[i][1] = v.y;
+            } else if constexpr (SB == 4) cur[i][0] = __ldg(reinterpret_cast<const uint32_t *>(src));
+            else cur[i][0] = __ldg(reinterpret_cast<const uint16_t *>(src));
+        };
+        auto fetch_params = [&](int t) {
+            const int64_t at = ((int64_t)t * (kTile / kGroup) + w) * D + 8 * chunk;
+            const float4 *s4 = reinterpret_cast<const float4 *>(ks + at), *z4 = reinterpret_cast<const float4 *>(kz + at);
             ns[0] = __ldg(s4); ns[1] = __ldg(s4 + 1);
             nz[0] = __ldg(z4); nz[1] = __ldg(z4 + 1);
         };
-        if (n_tiles > 0) fetch(t_lo);
+        if (here(t_lo)) {
+            fetch_params(t_lo);
+#pragma unroll
+            for (int i = 0; i < N; ++i) fetch_codes(t_lo, i);
+        }
         for (int i = 0; i < n_tiles; ++i) {
             const int t = t_lo + i, stage = i & 1;
             uint8_t *dst = smem + L::K + stage * L::TILE;
-            const bool packed = t < p.tiles_packed;
-            if (packed) {
-                const bool some = t * kTile + w * kGroup < st.n_quant;
-                uint32_t cur[N][W];
+            if (t < p.tiles_packed) {
+                const bool some = here(t), more = here(t + 1);
                 const float sc[8] = {ns[0].x, ns[0].y, ns[0].z, ns[0].w, ns[1].x, ns[1].y, ns[1].z, ns[1].w};
                 const float zz[8] = {nz[0].x, nz[0].y, nz[0].z, nz[0].w, nz[1].x, nz[1].y, nz[1].z, nz[1].w};
                 float ze[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) ze[k] = fmaf(-Codes<SB>::kBase, sc[k], zz[k]);
-#pragma unroll
-                for (int k = 0; k < N; ++k)
-#pragma unroll
-                    for (int j = 0; j < W; ++j) cur[k][j] = next[k][j];
-                if (i + 1 < n_tiles) fetch(t + 1);
+                if (more) fetch_params(t + 1);
                 if (i >= 2 && !wait(kKEmpty + stage, ((i >> 1) - 1) & 1)) break;
 #pragma unroll
-                for (int k = 0; k < N; ++k)
+                for (int k = 0; k < N; ++k) {
                     *reinterpret_cast<uint4 *>(dst + L::at(w * kGroup + TPL * k + sub, chunk)) = some ? decode8<SB>(cur[k], sc, ze) : zero4();
+                    if (more) fetch_codes(t + 1, k);
+                }
             } else {
                 if (i >= 2 && !wait(kKEmpty + stage, ((i >> 1) - 1) & 1)) break;
                 const int r0 = (t - p.tiles_packed) * kTile + w * kGroup;
-#pragma unroll 4
+#pragma unroll 2
                 for (int k = 0; k < N; ++k) {
                     const int row = r0 + TPL * k + sub;
                     uint4 v = zero4();
@@ -412,51 +440,39 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
         const uint8_t *codes = st.v_codes + hk * st.v_codes_stride_bh;
         const float *vs = st.v_scale + hk * st.v_param_stride_bh, *vz = st.v_zero + hk * st.v_param_stride_bh;
         const T *exact = reinterpret_cast<const T *>(st.v_res) + hk * st.res_stride_bh;
-        uint32_t next[N][W];
-        float ns[N], nz[N];
-        auto fetch = [&](int t) {
-            if (t >= p.tiles_packed) return;
+        uint32_t cur[N][W];   // as for the keys
+        float sc[N], ze[N];
+        auto here = [&](int t, int i) { return t < min(t_hi, p.tiles_packed) && t * kTile + i * TPI + tok < st.n_quant; };
+        auto fetch = [&](int t, int i) {
+            const int64_t slot = (int64_t)t * kTile + i * TPI + tok;
+            const uint8_t *src = codes + slot * RB + grp * (4 * SB);
+            if constexpr (W == 2) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(src));
+                cur[i][0] = v.x; cur[i][1] = v.y;
+            } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int64_t slot = (int64_t)t * kTile + i * TPI + tok;
-                if (slot >= st.n_quant) break;
-                const uint8_t *src = codes + slot * RB + grp * (4 * SB);
-                if constexpr (W == 2) {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(src));
-                    next[i][0] = v.x; next[i][1] = v.y;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < W; j += 4) {
-                        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src) + j / 4);
-                        next[i][j] = v.x; next[i][j + 1] = v.y; next[i][j + 2] = v.z; next[i][j + 3] = v.w;
-                    }
+                for (int j = 0; j < W; j += 4) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src) + j / 4);
+                    cur[i][j] = v.x; cur[i][j + 1] = v.y; cur[i][j + 2] = v.z; cur[i][j + 3] = v.w;
                 }
-                ns[i] = __ldg(vs + slot * GV + grp);
-                nz[i] = __ldg(vz + slot * GV + grp);
             }
+            sc[i] = __ldg(vs + slot * GV + grp);
+            ze[i] = __ldg(vz + slot * GV + grp);
         };
-        if (n_tiles > 0) fetch(t_lo);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (here(t_lo, i)) fetch(t_lo, i);
         for (int i = 0; i < n_tiles; ++i) {
             const int t = t_lo + i, stage = i & 1;
             uint8_t *dst = smem + L::V + stage * L::TILE;
             if (t < p.tiles_packed) {
-                uint32_t cur[N][W];
-                float sc[N], ze[N];
-#pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    sc[k] = ns[k];
-                    ze[k] = fmaf(-Codes<SB>::kBase, ns[k], nz[k]);
-#pragma unroll
-                    for (int j = 0; j < W; ++j) cur[k][j] = next[k][j];
-                }
-                if (i + 1 < n_tiles) fetch(t + 1);
                 if (i >= 2 && !wait(kVEmpty + stage, ((i >> 1) - 1) & 1)) break;
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
                     const int row = k * TPI + tok;
-                    const bool some = t * kTile + row < st.n_quant;
-                    const float s8[8] = {sc[k], sc[k], sc[k], sc[k], sc[k], sc[k], sc[k], sc[k]};
-                    const float z8[8] = {ze[k], ze[k], ze[k], ze[k], ze[k], ze[k], ze[k], ze[k]};
+                    const bool some = here(t, k);
+                    const float sk = sc[k], zk = fmaf(-Codes<SB>::kBase, sc[k], ze[k]);
+                    const float s8[8] = {sk, sk, sk, sk, sk, sk, sk, sk}, z8[8] = {zk, zk, zk, zk, zk, zk, zk, zk};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t wd[SB == 8 ? 2 : 1];
@@ -465,11 +481,12 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
                         else wd[0] = cur[k][j / 2] >> (16 * (j & 1));
                         *reinterpret_cast<uint4 *>(dst + L::at(row, 4 * grp + j)) = some ? decode8<SB>(wd, s8, z8) : zero4();
                     }
+                    if (here(t + 1, k)) fetch(t + 1, k);
                 }
             } else {
                 if (i >= 2 && !wait(kVEmpty + stage, ((i >> 1) - 1) & 1)) break;
                 const int r0 = (t - p.tiles_packed) * kTile;
-#pragma unroll
+#pragma unroll 1
                 for (int k = 0; k < N; ++k) {
                     const int row = k * TPI + tok;
 #pragma unroll
@@ -489,16 +506,19 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
         }
     } else if (lane == 0) {
         // ---- the MMAs, all by one thread, in order ------------------------------------------------------
-        const uint32_t sq = smem_u32(smem + L::Q), sk = smem_u32(smem + L::K), sv = smem_u32(smem + L::V);
+        // (a descriptor's low word holds the address in 16-byte units: stages and k-steps are added to it)
+        const uint64_t dq = make_desc(smem_u32(smem + L::Q), 16, 1024), dk = make_desc(smem_u32(smem + L::K), 16, 1024);
+        const uint64_t dv = make_desc(smem_u32(smem + L::V), L::HALF, 1024);
         auto qk = [&](int j) {
             const int s = j & 1, t = TILES == 2 ? j >> 1 : j, stage = t & 1;
             if ((TILES == 1 || s == 0) && !wait_one(kKFull + stage, (t >> 1) & 1)) return;
             fence_after();
+            const uint64_t a = dq + (TILES == 2 ? s * (L::TILE >> 4) : 0), b = dk + stage * (L::TILE >> 4);
+            const uint32_t d = tmem + 128 * s;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-                const uint32_t off = (uint32_t)((k >> 2) * L::HALF + (k & 3) * 32);
-                mma_ss(tmem_s[s], make_desc(sq + (TILES == 2 ? s * L::TILE : 0) + off, 16, 1024), make_desc(sk + stage * L::TILE + off, 16, 1024),
-                       make_idesc(kTile, false), k > 0);
+                const uint32_t off = (uint32_t)((k >> 2) * L::HALF + (k & 3) * 32) >> 4;
+                mma_ss(d, a + off, b + off, make_idesc(kTile, false), k > 0);
             }
             mma_commit(bar(kSFull + s));
             if (TILES == 1 || s == 1) mma_commit(bar(kKEmpty + stage));
@@ -508,16 +528,16 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
             if ((TILES == 1 || s == 0) && !wait_one(kVFull + stage, (t >> 1) & 1)) return;
             if (!wait_one(kPReady + s, (j >> 1) & 1)) return;
             fence_after();
+            const uint64_t b = dv + stage * (L::TILE >> 4);
+            const uint32_t d = tmem + 256 + 128 * s, a = tmem + 128 * s;
 #pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
-                mma_ts(tmem_o[s], tmem_s[s] + 8 * k, make_desc(sv + stage * L::TILE + k * 2048, L::HALF, 1024), make_idesc(D, true), j >= 2 || k > 0);
+            for (int k = 0; k < kTile / 16; ++k) mma_ts(d, a + 8 * k, b + k * (2048 >> 4), make_idesc(D, true), j >= 2 || k > 0);
             if (TILES == 1 || s == 1) mma_commit(bar(kVEmpty + stage));
             if (j + 2 >= n_steps) mma_commit(bar(kODone + s));
         };
-        if (n_steps > 0) qk(0);
-        if (n_steps > 1) qk(1);
-        for (int j = 0; j < n_steps && !gave_up; ++j) {
-            pv(j);
+#pragma unroll 1
+        for (int j = -2; j < n_steps && !gave_up; ++j) {
+            if (j >= 0) pv(j);
             if (j + 2 < n_steps && !gave_up) qk(j + 2);
         }
         if (gave_up) {  // MMAs in flight still use shared and tensor memory
