@@ -79,6 +79,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
                  "l"(b), "r"(idesc), "r"(accumulate)
                  : "memory");
 }
+// true in one lane of the (converged) warp, always the same one
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -105,34 +111,11 @@ __device__ __forceinline__ void tmem_ld_wait(float (&v)[32]) {
                  :
                  : "memory");
 }
-// The same for an array loaded before a tmem_ld_wait of another (both statements keep their order).
-__device__ __forceinline__ void tmem_pin(float (&v)[32]) {
-    asm volatile(""
-                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
-                   "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]),
-                   "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
-                   "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
-                 :
-                 : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
                  "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
-    uint32_t r[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
-        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-          "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-          "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
-        : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -143,13 +126,34 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// Columns from `n` on (of 64 in two arrays) become `x`.
-__device__ __forceinline__ void drop_from(float (&v)[32], float (&w)[32], int n, float x) {
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                 "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+// 8 columns of this lane times f: float32 outputs, or pairs of half weights
+__device__ __forceinline__ void scale_o(uint32_t addr, float f) {
+    uint32_t r[8];
+    tmem_ld8(addr, r);
 #pragma unroll
-    for (int k = 0; k < 32; ++k) {
-        v[k] = k < n ? v[k] : x;
-        w[k] = 32 + k < n ? w[k] : x;
+    for (int k = 0; k < 8; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * f);
+    tmem_st8(addr, r);
+}
+__device__ __forceinline__ void scale_p(uint32_t addr, float f) {
+    uint32_t r[8];
+    tmem_ld8(addr, r);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&r[k]));
+        r[k] = pack_f16(x.x * f, x.y * f);
     }
+    tmem_st8(addr, r);
 }
 
 struct PrefixParams {
@@ -180,15 +184,16 @@ enum { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPReady = 1
 
 __device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
 
-// 8 neighbouring codes of a row (SB bytes) as 8 halves
+// 8 neighbouring codes of a row (SB bytes) as 8 halves; scale and zero - BASE * scale of channel pairs
 template <int SB>
-__device__ __forceinline__ uint4 decode8(const uint32_t (&w)[SB == 8 ? 2 : 1], const float (&sc)[8], const float (&ze)[8]) {
+__device__ __forceinline__ uint4 decode8(const uint32_t (&w)[SB == 8 ? 2 : 1], const float2 (&sc)[4], const float2 (&ze)[4]) {
     uint32_t r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         constexpr int per = Codes<SB>::kPerWord;
-        r[i] = pack_f16(fmaf(Codes<SB>::get(w[2 * i / per], 2 * i % per), sc[2 * i], ze[2 * i]),
-                        fmaf(Codes<SB>::get(w[(2 * i + 1) / per], (2 * i + 1) % per), sc[2 * i + 1], ze[2 * i + 1]));
+        const float2 c = make_float2(Codes<SB>::get(w[2 * i / per], 2 * i % per), Codes<SB>::get(w[(2 * i + 1) / per], (2 * i + 1) % per));
+        const float2 v = fma2(c, sc[i], ze[i]);
+        r[i] = pack_f16(v.x, v.y);
     }
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
@@ -258,10 +263,6 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
         if (!gave_up) gave_up = !__all_sync(0xffffffffu, mbar_wait(bar(b), parity));
         return !gave_up;
     };
-    auto wait_one = [&](int b, uint32_t parity) {  // by the one thread that issues the MMAs
-        if (!gave_up && !mbar_wait(bar(b), parity)) gave_up = true;
-        return !gave_up;
-    };
 
     if (warp < 8) {
         // ---- softmax: thread = row -----------------------------------------------------------------
@@ -275,71 +276,58 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
             const int nv = t < p.tiles_packed ? min(kTile, st.n_quant - t * kTile) : min(kTile, st.n_res - (t - p.tiles_packed) * kTile);
             if (!wait(kSFull + s, i & 1)) break;
             fence_after();
-            float mx = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < kTile; c += 64) {
-                float v[32], w[32];
-                tmem_ld32(ts + c, v);
-                tmem_ld32(ts + c + 32, w);
-                tmem_ld_wait(v);
-                tmem_pin(w);
-                if (nv < c + 64) drop_from(v, w, nv - c, -INFINITY);
-                float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+            float2 sum[2] = {};
+            // 32 scores (already loaded) to weights; their largest may first raise m
+            auto chunk = [&](int c, float (&v)[32]) {
+                if (nv < c + 32) {
 #pragma unroll
-                for (int k = 0; k < 32; k += 2) {
-                    m4[(k >> 1) & 1] = max3(m4[(k >> 1) & 1], v[k], v[k + 1]);
-                    m4[2 + ((k >> 1) & 1)] = max3(m4[2 + ((k >> 1) & 1)], w[k], w[k + 1]);
+                    for (int k = 0; k < 32; ++k) v[k] = c + k < nv ? v[k] : -INFINITY;
                 }
-                mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
-            }
-            mx *= p.scale_log2;
-            const bool raise = mx > m + kLazy || (m == -INFINITY && mx != -INFINITY);
-            if (__any_sync(0xffffffffu, raise)) {
-                const float mn = raise ? mx : m;
-                const float f = m == -INFINITY ? 0.f : ex2(m - mn);
-                m = mn;
-                l *= f;
-                if (i > 0) {
-#pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        float v[32];
-                        tmem_ld32(to + 32 * c, v);
-                        tmem_ld_wait(v);
+                float mx = max3(v[0], v[1], v[2]), m1 = max3(v[3], v[4], v[5]);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) v[k] *= f;
-                        tmem_st32(to + 32 * c, v);
+                for (int k = 6; k < 30; k += 4) {
+                    mx = max3(mx, v[k], v[k + 1]);
+                    m1 = max3(m1, v[k + 2], v[k + 3]);
+                }
+                mx = fmaxf(max3(mx, m1, v[30]), v[31]) * p.scale_log2;
+                if (__any_sync(0xffffffffu, mx > m + kLazy)) {
+                    const float mn = mx > m + kLazy ? mx : m, f = m == -INFINITY ? 0.f : mn == m ? 1.f : ex2(m - mn);
+                    m = mn;
+                    l *= f;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) { sum[k].x *= f; sum[k].y *= f; }
+                    if (i > 0) {
+#pragma unroll 1
+                        for (int k = 0; k < D; k += 8) scale_o(to + k, f);
                     }
-                }
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-            float sum[4] = {};
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 #pragma unroll 1
-            for (int c = 0; c < kTile; c += 64) {
-                float v[32], w[32];
-                tmem_ld32(ts + c, v);
-                tmem_ld32(ts + c + 32, w);
-                tmem_ld_wait(v);
-                tmem_pin(w);
-#pragma unroll
-                for (int k = 0; k < 32; ++k) v[k] = ex2(fmaf(v[k], p.scale_log2, -base));
-#pragma unroll
-                for (int k = 0; k < 32; ++k) w[k] = ex2(fmaf(w[k], p.scale_log2, -base));
-                if (nv < c + 64) drop_from(v, w, nv - c, 0.f);
+                    for (int k = 0; k < c / 2; k += 8) scale_p(ts + k, f);
+                }
+                const float base = m == -INFINITY ? 0.f : -m;
                 uint32_t r[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    sum[k & 3] += v[2 * k] + v[2 * k + 1];
-                    r[k] = pack_f16(v[2 * k], v[2 * k + 1]);
+                    float2 x = fma2(make_float2(v[2 * k], v[2 * k + 1]), make_float2(p.scale_log2, p.scale_log2), make_float2(base, base));
+                    x.x = ex2(x.x);
+                    x.y = ex2(x.y);
+                    sum[k & 1] = add2(sum[k & 1], x);
+                    r[k] = pack_f16(x.x, x.y);
                 }
                 tmem_st16(ts + c / 2, r);  // (over scores that have been read)
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    sum[k & 3] += w[2 * k] + w[2 * k + 1];
-                    r[k] = pack_f16(w[2 * k], w[2 * k + 1]);
-                }
-                tmem_st16(ts + c / 2 + 16, r);
+            };
+            float v[32], w[32];
+            tmem_ld32(ts, v);
+#pragma unroll 1
+            for (int c = 0; c < kTile; c += 64) {
+                tmem_ld_wait(v);
+                tmem_ld32(ts + c + 32, w);
+                chunk(c, v);
+                tmem_ld_wait(w);
+                if (c + 64 < kTile) tmem_ld32(ts + c + 64, v);
+                chunk(c + 32, w);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             fence_before();
             __syncwarp();
@@ -400,17 +388,22 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
             uint8_t *dst = smem + L::K + stage * L::TILE;
             if (t < p.tiles_packed) {
                 const bool some = here(t), more = here(t + 1);
-                const float sc[8] = {ns[0].x, ns[0].y, ns[0].z, ns[0].w, ns[1].x, ns[1].y, ns[1].z, ns[1].w};
-                const float zz[8] = {nz[0].x, nz[0].y, nz[0].z, nz[0].w, nz[1].x, nz[1].y, nz[1].z, nz[1].w};
-                float ze[8];
+                const float2 sc[4] = {{ns[0].x, ns[0].y}, {ns[0].z, ns[0].w}, {ns[1].x, ns[1].y}, {ns[1].z, ns[1].w}};
+                const float2 zz[4] = {{nz[0].x, nz[0].y}, {nz[0].z, nz[0].w}, {nz[1].x, nz[1].y}, {nz[1].z, nz[1].w}};
+                float2 ze[4];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) ze[k] = fmaf(-Codes<SB>::kBase, sc[k], zz[k]);
+                for (int k = 0; k < 4; ++k) ze[k] = fma2(make_float2(-Codes<SB>::kBase, -Codes<SB>::kBase), sc[k], zz[k]);
                 if (more) fetch_params(t + 1);
                 if (i >= 2 && !wait(kKEmpty + stage, ((i >> 1) - 1) & 1)) break;
+                if (some) {
 #pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    *reinterpret_cast<uint4 *>(dst + L::at(w * kGroup + TPL * k + sub, chunk)) = some ? decode8<SB>(cur[k], sc, ze) : zero4();
-                    if (more) fetch_codes(t + 1, k);
+                    for (int k = 0; k < N; ++k) {
+                        *reinterpret_cast<uint4 *>(dst + L::at(w * kGroup + TPL * k + sub, chunk)) = decode8<SB>(cur[k], sc, ze);
+                        if (more) fetch_codes(t + 1, k);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int k = 0; k < N; ++k) *reinterpret_cast<uint4 *>(dst + L::at(w * kGroup + TPL * k + sub, chunk)) = zero4();
                 }
             } else {
                 if (i >= 2 && !wait(kKEmpty + stage, ((i >> 1) - 1) & 1)) break;
@@ -472,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
                     const int row = k * TPI + tok;
                     const bool some = here(t, k);
                     const float sk = sc[k], zk = fmaf(-Codes<SB>::kBase, sc[k], ze[k]);
-                    const float s8[8] = {sk, sk, sk, sk, sk, sk, sk, sk}, z8[8] = {zk, zk, zk, zk, zk, zk, zk, zk};
+                    const float2 s8[4] = {{sk, sk}, {sk, sk}, {sk, sk}, {sk, sk}}, z8[4] = {{zk, zk}, {zk, zk}, {zk, zk}, {zk, zk}};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t wd[SB == 8 ? 2 : 1];
@@ -504,36 +497,44 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kVFull + stage));
         }
-    } else if (lane == 0) {
+    } else {
         // ---- the MMAs, all by one thread, in order ------------------------------------------------------
+        // (the whole warp walks through the loop, so that descriptors stay in uniform registers)
+        const bool elected = elect_one();
         // (a descriptor's low word holds the address in 16-byte units: stages and k-steps are added to it)
         const uint64_t dq = make_desc(smem_u32(smem + L::Q), 16, 1024), dk = make_desc(smem_u32(smem + L::K), 16, 1024);
         const uint64_t dv = make_desc(smem_u32(smem + L::V), L::HALF, 1024);
         auto qk = [&](int j) {
             const int s = j & 1, t = TILES == 2 ? j >> 1 : j, stage = t & 1;
-            if ((TILES == 1 || s == 0) && !wait_one(kKFull + stage, (t >> 1) & 1)) return;
+            if ((TILES == 1 || s == 0) && !wait(kKFull + stage, (t >> 1) & 1)) return;
             fence_after();
             const uint64_t a = dq + (TILES == 2 ? s * (L::TILE >> 4) : 0), b = dk + stage * (L::TILE >> 4);
             const uint32_t d = tmem + 128 * s;
+            if (elected) {
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                const uint32_t off = (uint32_t)((k >> 2) * L::HALF + (k & 3) * 32) >> 4;
-                mma_ss(d, a + off, b + off, make_idesc(kTile, false), k > 0);
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (uint32_t)((k >> 2) * L::HALF + (k & 3) * 32) >> 4;
+                    mma_ss(d, a + off, b + off, make_idesc(kTile, false), k > 0);
+                }
+                mma_commit(bar(kSFull + s));
+                if (TILES == 1 || s == 1) mma_commit(bar(kKEmpty + stage));
             }
-            mma_commit(bar(kSFull + s));
-            if (TILES == 1 || s == 1) mma_commit(bar(kKEmpty + stage));
+            __syncwarp();
         };
         auto pv = [&](int j) {
             const int s = j & 1, t = TILES == 2 ? j >> 1 : j, stage = t & 1;
-            if ((TILES == 1 || s == 0) && !wait_one(kVFull + stage, (t >> 1) & 1)) return;
-            if (!wait_one(kPReady + s, (j >> 1) & 1)) return;
+            if ((TILES == 1 || s == 0) && !wait(kVFull + stage, (t >> 1) & 1)) return;
+            if (!wait(kPReady + s, (j >> 1) & 1)) return;
             fence_after();
             const uint64_t b = dv + stage * (L::TILE >> 4);
             const uint32_t d = tmem + 256 + 128 * s, a = tmem + 128 * s;
+            if (elected) {
 #pragma unroll
-            for (int k = 0; k < kTile / 16; ++k) mma_ts(d, a + 8 * k, b + k * (2048 >> 4), make_idesc(D, true), j >= 2 || k > 0);
-            if (TILES == 1 || s == 1) mma_commit(bar(kVEmpty + stage));
-            if (j + 2 >= n_steps) mma_commit(bar(kODone + s));
+                for (int k = 0; k < kTile / 16; ++k) mma_ts(d, a + 8 * k, b + k * (2048 >> 4), make_idesc(D, true), j >= 2 || k > 0);
+                if (TILES == 1 || s == 1) mma_commit(bar(kVEmpty + stage));
+                if (j + 2 >= n_steps) mma_commit(bar(kODone + s));
+            }
+            __syncwarp();
         };
 #pragma unroll 1
         for (int j = -2; j < n_steps && !gave_up; ++j) {
@@ -541,7 +542,8 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
             if (j + 2 < n_steps && !gave_up) qk(j + 2);
         }
         if (gave_up) {  // MMAs in flight still use shared and tensor memory
-            mma_commit(bar(kDrain));
+            if (elected) mma_commit(bar(kDrain));
+            __syncwarp();
             mbar_wait(bar(kDrain), 0);
         }
     }
