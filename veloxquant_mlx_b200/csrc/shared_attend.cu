@@ -17,8 +17,9 @@ namespace vq {
 namespace {
 
 constexpr int kGroup = 32;
-constexpr int kRowTile = 16;
+constexpr int kHalf = 16;   // exact rows of one work item
 constexpr int kWarps = 4;
+constexpr int kStages = 2;
 
 struct RowsParams {
     const void *q;
@@ -32,48 +33,81 @@ struct RowsParams {
     int prefix_blocks;             // blocks [0, prefix_blocks) work on the prefix, the rest on own tokens
 };
 
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    return r;
+}
+// 16 bytes from global to shared memory; zeros when `live` is false
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
 template <int N>
-__device__ __forceinline__ void load_words(uint32_t (&w)[N], const void *p) {
+__device__ __forceinline__ void lds(uint32_t (&w)[N], const uint8_t *p) {
     if constexpr (N % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p) + i / 4);
+            const uint4 v = *reinterpret_cast<const uint4 *>(p + 4 * i);
             w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
         }
     } else if constexpr (N == 2) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
         w[0] = v.x; w[1] = v.y;
     } else {
-        w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
     }
 }
 
-// One CTA: 16 query rows of one unit (kv head of the prefix, or kv head of one request's own store)
-// over one split of its 32-token groups, four warps taking groups in turn. Tensor cores by
-// m16n8k16 with query rows on M: 16 rows are what the own part has (H_q/H_kv heads, a few drafted
-// tokens), a tile a tcgen05 MMA would leave seven eighths empty. Codes go straight from global
-// memory to registers: the order of channels inside an MMA is free, so a thread's B fragment of
-// QK^T is one contiguous run of D/4 channels of a token, and of PV a run of D/8 channels.
-// Bound by HBM for few rows in principle; by instruction issue in practice (about 3 instructions a code).
-template <int D, int SB, typename T>
-__global__ void __launch_bounds__(kWarps * 32)
-shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
-    constexpr int CH = D / 4, CN = D / 8, KS = D / 16;   // channels a thread owns for K, for V; k-steps of QK^T
-    constexpr int KW = CH * SB / 32;                     // words of a thread's key codes of one token
-    constexpr int VB = CN * SB;                          // bits of a thread's value codes of one token
-    constexpr int VW = VB >= 32 ? VB / 32 : 1;
-    constexpr int GV = D / kGroup;
-    __shared__ float sh_o[kWarps][kRowTile][D + 4];
-    __shared__ float sh_m[kWarps][kRowTile], sh_l[kWarps][kRowTile];
+// One stage of a warp's ring: a packed group (key codes | value codes | key scales | key zeros | value
+// scales | value zeros) or 16 exact rows (keys | values).
+template <int D, int SB>
+struct Stage {
+    static constexpr int RB = D * SB / 8, GV = D / kGroup;
+    static constexpr int KC = 0, VC = KC + kGroup * RB, KS = VC + kGroup * RB, KZ = KS + 4 * D, VS = KZ + 4 * D, VZ = VS + kGroup * GV * 4;
+    static constexpr int PACKED = VZ + kGroup * GV * 4;
+    static constexpr int ROW = 2 * D, VR = kHalf * ROW, EXACT = 2 * kHalf * ROW;
+    static constexpr int BYTES = PACKED > EXACT ? PACKED : EXACT;
+    // Key scales and zeros: the four lanes of a quad read 16-byte chunks that are 128 (64) bytes apart: the
+    // chunk's place in its 128-byte line is turned so that they fall on different banks.
+    __device__ static __forceinline__ int param_chunk(int j) { return j ^ ((j >> 3) * (D == 128 ? 2 : 1)); }
+    // Exact rows: chunk j of row r
+    __device__ static __forceinline__ int row_chunk(int r, int j) { return r * ROW + ((j ^ (r & 7)) << 4); }
+};
 
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int g8 = lane >> 2, l4 = lane & 3;
+// One CTA: 8 or 16 query rows (NT tiles of 8) of one unit (kv head of the prefix, or kv head of one
+// request's own store) over one split of its tokens. Tensor cores by m16n8k16 with tokens (QK^T) and
+// channels (PV) on M and query rows on N: the own part has few rows (H_q/H_kv heads, a few drafted
+// tokens), of which a tcgen05 tile of 128 would waste nearly all.
+// Each warp takes work items in turn (a packed group of 32 tokens, or 16 exact rows), copied by cp.async
+// into its own two-stage ring, so that an item is in flight while the one before is decoded; no
+// synchronisation between warps until the end. The order of channels and of tokens inside an MMA is
+// free: a lane's K fragments are one run of D/4 channels of a token, its V fragments one run of D/8
+// channels, and the four tokens of a quad lie in rows whose banks differ.
+// Bound by HBM in principle (6 KB a group at 4 bits against about 760 instructions a warp).
+template <int D, int SB, typename T, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
+shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
+    using S = Stage<D, SB>;
+    constexpr int CH = D / 4, CN = D / 8, KS = D / 16;   // channels a lane owns for K, for V; k-steps of QK^T
+    constexpr int MT = CN / 2;                           // 16-channel tiles of the output
+    constexpr int KW = CH * SB / 32;                     // words of a lane's key codes of one token
+    constexpr int VB = CN * SB;                          // bits of a lane's value codes of one token
+    constexpr int VW = VB >= 32 ? VB / 32 : 1;
+    constexpr int GV = S::GV, RB = S::RB;
+    constexpr int ROWS = 8 * NT;
+    constexpr float BASE = Codes<SB>::kBase;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float sh_m[kWarps][ROWS], sh_l[kWarps][ROWS];
+
+    const int lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int g8 = lane >> 2, c4 = lane & 3;
+    const int tau = (g8 >> 1) | ((g8 & 1) << 2);         // token of row g8 of a key tile
     const bool is_prefix = (int)blockIdx.x < p.prefix_blocks;
     int blk = is_prefix ? blockIdx.x : blockIdx.x - p.prefix_blocks;
     const int ns = is_prefix ? p.np : p.no;
@@ -86,186 +120,265 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
     const vq_kivi_rows &st = is_prefix ? p.prefix : p.own;
     const int per_req = p.G * p.S_q;                     // query rows of one request and kv head
     const int n_rows = is_prefix ? p.B * per_req : per_req;
+    auto out_row = [&](int r) {                          // output row (= row of q) of the unit's query row r
+        const int b = is_prefix ? r / per_req : b_own, rem = is_prefix ? r - b * per_req : r;
+        return ((int64_t)b * p.H_q + (int64_t)hk * p.G) * p.S_q + rem;
+    };
 
-    const int64_t n_slots = (int64_t)st.n_quant + st.n_res;
-    const int ng = st.n_quant / kGroup;                  // packed groups; exact rows start at slot 32 * ng
-    const int groups = ng + (st.n_res + kGroup - 1) / kGroup;
-    const int first_slot = is_prefix || !p.own_start ? 0 : max(0, __ldg(p.own_start + b_own));
-    const int g_first = min(groups, first_slot / kGroup);
-    const int per_split = (groups - g_first + ns - 1) / ns;
-    const int g_lo = min(groups, g_first + split * per_split), g_hi = min(groups, g_lo + per_split);
+    const int n_slots = st.n_quant + st.n_res;
+    const int first_slot = is_prefix || !p.own_start ? 0 : min(n_slots, max(0, __ldg(p.own_start + b_own)));
+    const int ng = st.n_quant / kGroup;                  // packed items; exact rows start at slot 32 * ng
+    const int items = ng + (st.n_res + kHalf - 1) / kHalf;
+    const int i_first = first_slot < st.n_quant ? first_slot / kGroup : ng + (first_slot - st.n_quant) / kHalf;
+    const int per_split = (items - i_first + ns - 1) / ns;
+    const int i_lo = min(items, i_first + split * per_split), i_hi = min(items, i_lo + per_split);
 
-    // this thread's two query rows: output row (= row of q), and the first slot that they do not see
-    int64_t out_row[2];
-    int lim[2];
-    bool live[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = tile * kRowTile + g8 + 8 * i;
-        live[i] = r < n_rows;
-        const int rr = live[i] ? r : 0;
-        const int b = is_prefix ? rr / per_req : b_own, rem = is_prefix ? rr - b * per_req : rr;
-        out_row[i] = ((int64_t)b * p.H_q + (int64_t)hk * p.G) * p.S_q + rem;
-        lim[i] = !live[i] ? 0 : is_prefix || !p.causal ? (int)n_slots : (int)n_slots - p.S_q + rem % p.S_q + 1;
-    }
-
-    // Q: row g8 (+8), channels l4*CH ..
-    uint32_t qa[KS][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        uint32_t w[CH / 2] = {};
-        if (live[i]) load_words(w, reinterpret_cast<const T *>(p.q) + out_row[i] * D + l4 * CH);
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            qa[k][i] = as_f16x2<T>(w[2 * k]);
-            qa[k][2 + i] = as_f16x2<T>(w[2 * k + 1]);
-        }
-    }
-
-    float o[CN][4] = {};
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    uint8_t *ring = smem + warp * (kStages * S::BYTES);
+    const uint32_t ring_u32 = (uint32_t)__cvta_generic_to_shared(ring);
     const uint8_t *kc = st.k_codes + unit * st.k_codes_stride_bh, *vc = st.v_codes + unit * st.v_codes_stride_bh;
     const float *ks = st.k_scale + unit * st.k_param_stride_bh, *kz = st.k_zero + unit * st.k_param_stride_bh;
     const float *vs = st.v_scale + unit * st.v_param_stride_bh, *vz = st.v_zero + unit * st.v_param_stride_bh;
     const T *kr = reinterpret_cast<const T *>(st.k_res) + unit * st.res_stride_bh;
     const T *vr = reinterpret_cast<const T *>(st.v_res) + unit * st.res_stride_bh;
 
-    for (int grp = g_lo + warp; grp < g_hi; grp += kWarps) {
-        const bool packed = grp < ng;
-        const int slot0 = grp * kGroup;
-        float s[4][4] = {};
-        // ---- S = Q K^T -----------------------------------------------------------------------
-        if (packed) {
+    // Values of slots before first_slot and of rows behind the last enter the ring as zeros, so that
+    // whatever is stored there cannot reach the output (their scores are dropped below).
+    auto fetch = [&](int item, int stage) {
+        const uint32_t dst = ring_u32 + stage * S::BYTES;
+        if (item < ng) {
+            const int64_t slot0 = (int64_t)item * kGroup;
+            const uint8_t *k0 = kc + slot0 * RB, *v0 = vc + slot0 * RB;
+#pragma unroll
+            for (int j = lane; j < kGroup * RB / 16; j += 32) {
+                copy16(dst + S::KC + 16 * j, k0 + 16 * j, true);
+                copy16(dst + S::VC + 16 * j, v0 + 16 * j, true);
+            }
+            const float *s0 = ks + (int64_t)item * D, *z0 = kz + (int64_t)item * D;
+            if (D == 128 || lane < 16) {
+                copy16(dst + S::KS + 16 * S::param_chunk(lane), s0 + 4 * lane, true);
+                copy16(dst + S::KZ + 16 * S::param_chunk(lane), z0 + 4 * lane, true);
+                // (a 16-byte chunk holds the scales of one token (D = 128) or two; a padding token that
+                // shares a chunk with a live one is dealt with where values are decoded)
+                const bool live = slot0 + (4 * lane + 3) / GV >= first_slot;
+                copy16(dst + S::VS + 16 * lane, vs + slot0 * GV + 4 * lane, live);
+                copy16(dst + S::VZ + 16 * lane, vz + slot0 * GV + 4 * lane, live);
+            }
+        } else {
+            const int r0 = (item - ng) * kHalf;
+#pragma unroll
+            for (int j = lane; j < kHalf * (D / 8); j += 32) {
+                const int r = j / (D / 8), ch = j % (D / 8);
+                const bool in = r0 + r < st.n_res, seen = in && st.n_quant + r0 + r >= first_slot;
+                const int64_t at = in ? (int64_t)(r0 + r) * D + 8 * ch : 0;
+                copy16(dst + S::row_chunk(r, ch), kr + at, in);
+                copy16(dst + S::VR + S::row_chunk(r, ch), vr + at, seen);
+            }
+        }
+    };
+
+    // Q: row g8 of each tile, channels c4*CH ..
+    uint32_t qb[NT][CH / 2];
+    int lim[NT][2];  // first slot that rows 2*c4 and 2*c4 + 1 of a tile do not see
+    if (i_lo + warp < i_hi) fetch(i_lo + warp, 0);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = tile * ROWS + 8 * nt + g8;
+#pragma unroll
+        for (int i = 0; i < CH / 2; ++i) qb[nt][i] = 0u;
+        if (r < n_rows) {
+            const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(p.q) + out_row(r) * D + c4 * CH);
+#pragma unroll
+            for (int i = 0; i < CH / 8; ++i) {
+                const uint4 v = __ldg(src + i);
+                qb[nt][4 * i] = as_f16x2<T>(v.x); qb[nt][4 * i + 1] = as_f16x2<T>(v.y);
+                qb[nt][4 * i + 2] = as_f16x2<T>(v.z); qb[nt][4 * i + 3] = as_f16x2<T>(v.w);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int rr = tile * ROWS + 8 * nt + 2 * c4 + i;
+            lim[nt][i] = rr >= n_rows ? 0 : is_prefix || !p.causal ? n_slots : n_slots - p.S_q + rr % p.S_q + 1;
+        }
+    }
+
+    float o[NT][MT][4] = {};
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) { m[nt][0] = m[nt][1] = -INFINITY; l[nt][0] = l[nt][1] = 0.f; }
+
+    // Scores s[tile][2 * (16-token tile)...] of one item to weights: masks, running maxima, rescale of o.
+    // Returns the weights as B fragments of the item's 16-token steps.
+    auto softmax = [&](auto steps_c, float (&s)[NT][2][4], int slot0, uint32_t (&pb)[NT][2][2]) {
+        constexpr int STEPS = decltype(steps_c)::value;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int slot = slot0 + 16 * k + 8 * (c >> 1) + tau;
+                    s[nt][k][c] = slot >= first_slot && slot < lim[nt][c & 1] ? s[nt][k][c] * p.scale_log2 : -INFINITY;
+                    mx[c & 1] = fmaxf(mx[c & 1], s[nt][k][c]);
+                }
+            float base[2], f[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], d));
+                const float mn = fmaxf(m[nt][i], mx[i]);
+                base[i] = mn == -INFINITY ? 0.f : mn;
+                f[i] = ex2(m[nt][i] - base[i]);
+                m[nt][i] = mn;
+                l[nt][i] *= f[i];
+            }
+            if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+                for (int j = 0; j < MT; ++j) { o[nt][j][0] *= f[0]; o[nt][j][1] *= f[1]; o[nt][j][2] *= f[0]; o[nt][j][3] *= f[1]; }
+            }
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+                float e[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    e[c] = ex2(s[nt][k][c] - base[c & 1]);
+                    l[nt][c & 1] += e[c];
+                }
+                pb[nt][k][0] = transpose8x8(pack_f16(e[0], e[1]));
+                pb[nt][k][1] = transpose8x8(pack_f16(e[2], e[3]));
+            }
+        }
+    };
+
+    int stage = 0;
+    for (int item = i_lo + warp; item < i_hi; item += kWarps, stage ^= 1) {
+        if (item + kWarps < i_hi) fetch(item + kWarps, stage ^ 1);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
+        const uint8_t *buf = ring + stage * S::BYTES;
+        float s[NT][2][4] = {};
+        uint32_t pb[NT][2][2];
+        if (item < ng) {
+            // ---- S^T = K Q^T: rows of a key tile are tokens tau(g8), 8 + tau(g8) ----------------------
             uint32_t w[4][KW];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                load_words(w[j], kc + (int64_t)(slot0 + 8 * j + g8) * (D * SB / 8) + l4 * (CH * SB / 8));
+            for (int j = 0; j < 4; ++j) lds(w[j], buf + S::KC + (8 * j + tau) * RB + c4 * (CH * SB / 8));
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                const float4 sc = __ldg(reinterpret_cast<const float4 *>(ks + (int64_t)grp * D + l4 * CH + 4 * k));
-                const float4 ze = __ldg(reinterpret_cast<const float4 *>(kz + (int64_t)grp * D + l4 * CH + 4 * k));
-                const float z0 = fmaf(-Codes<SB>::kBase, sc.x, ze.x), z1 = fmaf(-Codes<SB>::kBase, sc.y, ze.y);
-                const float z2 = fmaf(-Codes<SB>::kBase, sc.z, ze.z), z3 = fmaf(-Codes<SB>::kBase, sc.w, ze.w);
+                const int at = 16 * S::param_chunk(c4 * (CH / 4) + k);
+                const float4 sc = *reinterpret_cast<const float4 *>(buf + S::KS + at), zz = *reinterpret_cast<const float4 *>(buf + S::KZ + at);
+                const float2 s0 = make_float2(sc.x, sc.y), s1 = make_float2(sc.z, sc.w), nb = make_float2(-BASE, -BASE);
+                const float2 z0 = fma2(nb, s0, make_float2(zz.x, zz.y)), z1 = fma2(nb, s1, make_float2(zz.z, zz.w));
+                uint32_t a[4][2];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t word = w[j][4 * k / Codes<SB>::kPerWord];
                     const int i0 = 4 * k % Codes<SB>::kPerWord;
-                    const uint32_t b0 = pack_f16(fmaf(Codes<SB>::get(word, i0), sc.x, z0), fmaf(Codes<SB>::get(word, i0 + 1), sc.y, z1));
-                    const uint32_t b1 = pack_f16(fmaf(Codes<SB>::get(word, i0 + 2), sc.z, z2), fmaf(Codes<SB>::get(word, i0 + 3), sc.w, z3));
-                    mma16816(s[j], qa[k], b0, b1);
+                    const float2 x = fma2(make_float2(Codes<SB>::get(word, i0), Codes<SB>::get(word, i0 + 1)), s0, z0);
+                    const float2 y = fma2(make_float2(Codes<SB>::get(word, i0 + 2), Codes<SB>::get(word, i0 + 3)), s1, z1);
+                    a[j][0] = pack_f16(x.x, x.y);
+                    a[j][1] = pack_f16(y.x, y.y);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma16816(s[nt][0], a[0][0], a[1][0], a[0][1], a[1][1], qb[nt][2 * k], qb[nt][2 * k + 1]);
+                    mma16816(s[nt][1], a[2][0], a[3][0], a[2][1], a[3][1], qb[nt][2 * k], qb[nt][2 * k + 1]);
+                }
+            }
+            const int slot0 = item * kGroup;
+            softmax(std::integral_constant<int, 2>{}, s, slot0, pb);
+            // ---- O^T += V^T P^T: a quad's tokens of a step are c4, c4 + 4, c4 + 8, c4 + 12 -------------
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                uint32_t x[4][VW];
+                float2 sc[4], ze[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const int tok = 16 * k + 4 * t + c4;
+                    const uint8_t *src = buf + S::VC + tok * RB + g8 * (VB / 8);
+                    if constexpr (VB == 16) x[t][0] = *reinterpret_cast<const uint16_t *>(src);
+                    else lds(x[t], src);
+                    const int at = 4 * (tok * GV + g8 * CN / kGroup);
+                    float a = *reinterpret_cast<const float *>(buf + S::VS + at), z = *reinterpret_cast<const float *>(buf + S::VZ + at);
+                    if (D == 64 && slot0 + tok < first_slot) a = z = 0.f;
+                    z = fmaf(-BASE, a, z);
+                    sc[t] = make_float2(a, a);
+                    ze[t] = make_float2(z, z);
+                }
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    float2 v[4];  // channels 2j, 2j + 1 of the four tokens
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const uint32_t word = x[t][2 * j / Codes<SB>::kPerWord];
+                        const int i0 = 2 * j % Codes<SB>::kPerWord;
+                        v[t] = fma2(make_float2(Codes<SB>::get(word, i0), Codes<SB>::get(word, i0 + 1)), sc[t], ze[t]);
+                    }
+                    const uint32_t a0 = pack_f16(v[0].x, v[1].x), a1 = pack_f16(v[0].y, v[1].y), a2 = pack_f16(v[2].x, v[3].x), a3 = pack_f16(v[2].y, v[3].y);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][j], a0, a1, a2, a3, pb[nt][k][0], pb[nt][k][1]);
                 }
             }
         } else {
-            const int row0 = slot0 - ng * kGroup;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t w[CH / 2] = {};
-                const int row = row0 + 8 * j + g8;
-                if (row < st.n_res) load_words(w, kr + (int64_t)row * D + l4 * CH);
+            for (int i = 0; i < CH / 8; ++i) {
+                uint32_t a[2][4];
+                lds(a[0], buf + S::row_chunk(tau, c4 * (CH / 8) + i));
+                lds(a[1], buf + S::row_chunk(8 + tau, c4 * (CH / 8) + i));
 #pragma unroll
-                for (int k = 0; k < KS; ++k) mma16816(s[j], qa[k], as_f16x2<T>(w[2 * k]), as_f16x2<T>(w[2 * k + 1]));
+                for (int k = 0; k < 4; ++k) { a[0][k] = as_f16x2<T>(a[0][k]); a[1][k] = as_f16x2<T>(a[1][k]); }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma16816(s[nt][0], a[0][0], a[1][0], a[0][1], a[1][1], qb[nt][4 * i], qb[nt][4 * i + 1]);
+                    mma16816(s[nt][0], a[0][2], a[1][2], a[0][3], a[1][3], qb[nt][4 * i + 2], qb[nt][4 * i + 3]);
+                }
             }
-        }
-        // ---- softmax: scores outside [first_slot, lim) are dropped whatever they are ------------
-        float mx[2] = {-INFINITY, -INFINITY};
+            softmax(std::integral_constant<int, 1>{}, s, st.n_quant + (item - ng) * kHalf, pb);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int slot = slot0 + 8 * j + 2 * l4 + (c & 1);
-                s[j][c] = slot >= first_slot && slot < lim[c >> 1] ? s[j][c] * p.scale_log2 : -INFINITY;
-                mx[c >> 1] = fmaxf(mx[c >> 1], s[j][c]);
-            }
-        float base[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-            const float mn = fmaxf(m[i], mx[i]);
-            base[i] = mn == -INFINITY ? 0.f : mn;
-            const float alpha = ex2(m[i] - base[i]);
-            m[i] = mn;
-            l[i] *= alpha;
-#pragma unroll
-            for (int j = 0; j < CN; ++j) { o[j][2 * i] *= alpha; o[j][2 * i + 1] *= alpha; }
-        }
-        uint32_t pa[2][4];  // P as A fragments of the two 16-token steps
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float e[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                e[c] = ex2(s[j][c] - base[c >> 1]);
-                l[c >> 1] += e[c];
-            }
-            pa[j >> 1][(j & 1) * 2] = pack_f16(e[0], e[1]);
-            pa[j >> 1][(j & 1) * 2 + 1] = pack_f16(e[2], e[3]);
-        }
-        // ---- O += P V: slots before first_slot may hold anything; their values enter as 0 --------
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            if (packed) {
-                uint32_t w[4][VW];
-                float sc[4], ze[4];
+            for (int i = 0; i < CN / 8; ++i) {
+                uint32_t x[4][4];
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    const int64_t slot = slot0 + 16 * kk + 2 * l4 + (t & 1) + 8 * (t >> 1);
-                    const uint8_t *src = vc + slot * (D * SB / 8) + g8 * (VB / 8);
-                    if constexpr (VB == 16) w[t][0] = __ldg(reinterpret_cast<const uint16_t *>(src));
-                    else load_words(w[t], src);
-                    const int64_t pi = slot * GV + g8 * CN / kGroup;
-                    const bool dead = slot < first_slot;
-                    sc[t] = dead ? 0.f : __ldg(vs + pi);
-                    ze[t] = dead ? 0.f : fmaf(-Codes<SB>::kBase, sc[t], __ldg(vz + pi));
+                    lds(x[t], buf + S::VR + S::row_chunk(4 * t + c4, g8 * (CN / 8) + i));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[t][k] = as_f16x2<T>(x[t][k]);
                 }
 #pragma unroll
-                for (int j = 0; j < CN; ++j) {
-                    float v[4];
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t a0 = __byte_perm(x[0][j], x[1][j], 0x5410), a1 = __byte_perm(x[0][j], x[1][j], 0x7632);
+                    const uint32_t a2 = __byte_perm(x[2][j], x[3][j], 0x5410), a3 = __byte_perm(x[2][j], x[3][j], 0x7632);
 #pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                        v[t] = fmaf(Codes<SB>::get(w[t][j / Codes<SB>::kPerWord], j % Codes<SB>::kPerWord), sc[t], ze[t]);
-                    mma16816(o[j], pa[kk], pack_f16(v[0], v[1]), pack_f16(v[2], v[3]));
-                }
-            } else {
-                uint32_t w[4][CN / 2];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const int slot = slot0 + 16 * kk + 2 * l4 + (t & 1) + 8 * (t >> 1);
-                    const int row = slot - ng * kGroup;
-#pragma unroll
-                    for (int i = 0; i < CN / 2; ++i) w[t][i] = 0u;
-                    if (row < st.n_res && slot >= first_slot) load_words(w[t], vr + (int64_t)row * D + g8 * CN);
-#pragma unroll
-                    for (int i = 0; i < CN / 2; ++i) w[t][i] = as_f16x2<T>(w[t][i]);
-                }
-#pragma unroll
-                for (int j = 0; j < CN; ++j) {
-                    const uint32_t sel = j & 1 ? 0x7632u : 0x5410u;
-                    mma16816(o[j], pa[kk], __byte_perm(w[0][j / 2], w[1][j / 2], sel), __byte_perm(w[2][j / 2], w[3][j / 2], sel));
+                    for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][4 * i + j], a0, a1, a2, a3, pb[nt][0][0], pb[nt][0][1]);
                 }
             }
         }
+        __syncwarp();  // the stage is read before it is refilled
     }
 
-    // ---- the four warps' partials into one record per row ----------------------------------------
+    // ---- the four warps' partials into one record per row (the rings are done with) ----------------
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    constexpr int LD = D + 4;
+    float *sh_o = reinterpret_cast<float *>(smem);  // [warp][row][channel]
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        const int r = g8 + 8 * i;
-        if (l4 == 0) { sh_m[warp][r] = m[i]; sh_l[warp][r] = l[i]; }
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < CN; ++j) {
-            sh_o[warp][r][2 * l4 * CN + j] = o[j][2 * i];
-            sh_o[warp][r][(2 * l4 + 1) * CN + j] = o[j][2 * i + 1];
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], d);
+            const int r = 8 * nt + 2 * c4 + i;
+            if (g8 == 0) { sh_m[warp][r] = m[nt][i]; sh_l[warp][r] = l[nt][i]; }
+            float *dst = sh_o + (warp * ROWS + r) * LD + g8 * CN;
+#pragma unroll
+            for (int j = 0; j < MT; ++j) *reinterpret_cast<float2 *>(dst + 2 * j) = make_float2(o[nt][j][i], o[nt][j][2 + i]);
         }
-    }
     __syncthreads();
     const int slot_of = (is_prefix ? 0 : p.np) + split;
-    for (int i = threadIdx.x; i < kRowTile * D / 4; i += kWarps * 32) {
+    for (int i = threadIdx.x; i < ROWS * D / 4; i += kWarps * 32) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
-        const int rr = tile * kRowTile + r;
-        if (rr >= n_rows) break;
+        if (tile * ROWS + r >= n_rows) break;
         float mm = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sh_m[w][r]);
@@ -275,14 +388,23 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
         for (int w = 0; w < kWarps; ++w) {
             const float f = ex2(sh_m[w][r] - bs);
             ll = fmaf(sh_l[w][r], f, ll);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) acc[c] = fmaf(sh_o[w][r][d + c], f, acc[c]);
+            const float4 v = *reinterpret_cast<const float4 *>(sh_o + (w * ROWS + r) * LD + d);
+            acc[0] = fmaf(v.x, f, acc[0]); acc[1] = fmaf(v.y, f, acc[1]); acc[2] = fmaf(v.z, f, acc[2]); acc[3] = fmaf(v.w, f, acc[3]);
         }
-        const int b = is_prefix ? rr / per_req : b_own, rem = is_prefix ? rr - b * per_req : rr;
-        const int64_t rec = (((int64_t)b * p.H_q + (int64_t)hk * p.G) * p.S_q + rem) * p.parts.n_splits + slot_of;
+        const int64_t rec = out_row(tile * ROWS + r) * p.parts.n_splits + slot_of;
         *reinterpret_cast<float4 *>(p.parts.o + rec * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         if (d == 0) *reinterpret_cast<float2 *>(p.parts.ml + rec * 2) = make_float2(mm, ll);
     }
+}
+
+template <int D, int SB, typename T, int NT>
+int32_t launch_rows(const RowsParams &p, unsigned blocks, cudaStream_t st) {
+    constexpr int ring = kWarps * kStages * Stage<D, SB>::BYTES, merge = kWarps * 8 * NT * (D + 4) * 4;
+    constexpr int smem = ring > merge ? ring : merge;
+    VQ_CHECK_CUDA(cudaFuncSetAttribute(shared_attend_rows_kernel<D, SB, T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    shared_attend_rows_kernel<D, SB, T, NT><<<blocks, kWarps * 32, smem, st>>>(p);
+    VQ_CHECK_LAUNCH("shared_attend_rows_kernel");
+    return VQ_OK;
 }
 
 // Joins the records of an output row: `ways` warps (1 or 4) take its records in turn, each lane D/32
@@ -350,6 +472,7 @@ __global__ void __launch_bounds__(128) shared_attend_merge_kernel(const SharedPa
 
 struct Plan {
     bool tc5;
+    int row_tile;  // query rows of a warp tile: 8 or 16
     int np, no;
     int prefix_tiles, own_tiles;
     int64_t rows;
@@ -370,8 +493,9 @@ int32_t plan_of(const vq_shared_attend_args &a, const DeviceInfo &di, Plan *out)
     const char *why = shared_prefix_tc5_supported(a);
     VQ_REQUIRE(a.variant != 2 || why == nullptr, VQ_ERR_SHAPE, "vq_kivi_shared_attend: tcgen05 kernel unavailable: %s", why);
     pl.tc5 = gp > 0 && why == nullptr && a.variant != 1;
-    pl.prefix_tiles = (int)ceil_div(a.B * per_req, kRowTile);
-    pl.own_tiles = (int)ceil_div(per_req, kRowTile);
+    pl.row_tile = (pl.tc5 ? per_req : a.B * per_req) > 8 ? 16 : 8;
+    pl.prefix_tiles = (int)ceil_div(a.B * per_req, pl.row_tile);
+    pl.own_tiles = (int)ceil_div(per_req, pl.row_tile);
     pl.no = go ? splits((int64_t)a.B * a.H_kv * pl.own_tiles, go) : 0;
     pl.np = !gp ? 0 : pl.tc5 ? shared_prefix_tc5_splits(a, di) : a.n_splits > 0 ? std::min({a.n_splits, gp, 64}) : splits((int64_t)a.H_kv * pl.prefix_tiles, gp);
     *out = pl;
@@ -438,10 +562,13 @@ int32_t launch_all(const vq_shared_attend_args &a, const Plan &pl, const DeviceI
         if (rc != VQ_OK) return rc;
     }
     if (blocks) {
-        if (a.store_bits == 2) shared_attend_rows_kernel<D, 2, T><<<(unsigned)blocks, kWarps * 32, 0, st>>>(p);
-        else if (a.store_bits == 4) shared_attend_rows_kernel<D, 4, T><<<(unsigned)blocks, kWarps * 32, 0, st>>>(p);
-        else shared_attend_rows_kernel<D, 8, T><<<(unsigned)blocks, kWarps * 32, 0, st>>>(p);
-        VQ_CHECK_LAUNCH("shared_attend_rows_kernel");
+        const bool wide = pl.row_tile == 16;
+        const unsigned nb = (unsigned)blocks;
+        int32_t rc;
+        if (a.store_bits == 2) rc = wide ? launch_rows<D, 2, T, 2>(p, nb, st) : launch_rows<D, 2, T, 1>(p, nb, st);
+        else if (a.store_bits == 4) rc = wide ? launch_rows<D, 4, T, 2>(p, nb, st) : launch_rows<D, 4, T, 1>(p, nb, st);
+        else rc = wide ? launch_rows<D, 8, T, 2>(p, nb, st) : launch_rows<D, 8, T, 1>(p, nb, st);
+        if (rc != VQ_OK) return rc;
     }
     const int ways = p.parts.n_splits > 8 ? 4 : 1;
     shared_attend_merge_kernel<D, T><<<(unsigned)ceil_div(pl.rows * ways, 4), 128, 0, st>>>(p.parts, pl.rows, ways, (T *)a.out, a.lse);
