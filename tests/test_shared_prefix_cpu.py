@@ -100,3 +100,15 @@ def test_struct_sizes_match_header(tmp_path):
     subprocess.run(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(exe)], check=True)
     out = subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()
     assert [int(x) for x in out] == [ctypes.sizeof(t) for t in (_lib.RotaryArgs, _lib.KiviRowsArgs, _lib.SharedAttendArgs)]
+    # the packed forms that the wrappers pass: the same bytes as the structures, field by field
+    for fmt, cls in ((_lib.ROTARY_PACK, _lib.RotaryArgs), (_lib.KIVI_ROWS_PACK, _lib.KiviRowsArgs)):
+        assert fmt.size == ctypes.sizeof(cls)
+    assert _lib.SHARED_ATTEND_HEAD.size == _lib.SharedAttendArgs.prefix.offset
+    assert _lib.SHARED_ATTEND_HEAD.size + 2 * _lib.KIVI_ROWS_PACK.size == _lib.SharedAttendArgs.workspace.offset
+    assert _lib.SHARED_ATTEND_HEAD.size + 2 * _lib.KIVI_ROWS_PACK.size + _lib.SHARED_ATTEND_TAIL.size == ctypes.sizeof(_lib.SharedAttendArgs)
+    r = _lib.RotaryArgs.from_buffer_copy(_lib.ROTARY_PACK.pack(*range(1, 37), 37.0, 38, 39, 40, 41))
+    assert list(r.x) == [1, 2, 3] and list(r.y_stride) == list(range(16, 25)) and list(r.heads) == [25, 26, 27] and r.dtype == 28
+    assert (r.B, r.S, r.D, r.rotary_dim, r.layout, r.inverse, r.positions, r.pos_bytes) == (29, 30, 31, 32, 33, 34, 35, 36)
+    assert (r.factor, r.pos_stride_b, r.pos_stride_s, r.pos_offset, r.turns) == (37.0, 38, 39, 40, 41)
+    k = _lib.KiviRowsArgs.from_buffer_copy(_lib.KIVI_ROWS_PACK.pack(*range(1, 16)))
+    assert (k.k_codes, k.v_res, k.k_codes_stride_bh, k.res_stride_bh, k.n_quant, k.n_res) == (1, 8, 9, 13, 14, 15)

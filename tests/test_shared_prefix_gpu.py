@@ -140,6 +140,10 @@ CASES = [
     (40, 8, 2, 1, 128, 4, BF, 1024, 100, 32, 20),
     (70, 4, 1, 1, 128, 4, HF, 640, 0, 0, 1),
     (9, 8, 1, 4, 128, 8, BF, 2048, 5, 32, 9),
+    (3, 8, 2, 40, 128, 4, BF, 640, 3, 160, 77),     # own tokens on the tensor-memory kernel, one and two row tiles
+    (2, 8, 2, 9, 128, 2, HF, 512, 0, 0, 40),
+    (2, 4, 4, 130, 64, 4, HF, 32, 9, 256, 130),
+    (1, 6, 1, 43, 128, 8, BF, 0, 0, 128, 128),
 ]
 
 
@@ -148,10 +152,14 @@ CASES = [
 def test_against_64_bits(case, variant):
     B, Hq, Hk, S, D, bits, dtype, pq, pr, oq, orr = case
     q = torch.randn(B, Hq, S, D, device=DEV, generator=_gen(1)).to(dtype)
+    if not pq + pr and variant == 2:
+        with pytest.raises(ValueError, match="needs a prefix"):
+            kivi_shared_prefix_attend(q, make_store(1, Hk, D, bits, 0, 0, dtype, 2)[0], None, 0.1, variant=2)
+        return
     check(q, make_store(1, Hk, D, bits, pq, pr, dtype, 2, spare=32), make_store(B, Hk, D, bits, oq, orr, dtype, 3, spare=64), D**-0.5, variant=variant)
 
 
-@pytest.mark.parametrize("S", [1, 4])
+@pytest.mark.parametrize("S", [1, 4, 33, 84])
 @pytest.mark.parametrize("causal", [True, False])
 def test_padding_on_the_left_and_what_it_holds(S, causal):
     B, H, D, n_own = 6, 2, 128, 64 + 20

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 
 import torch
@@ -183,6 +184,13 @@ class SharedAttendArgs(C.Structure):
     ]
 
 
+# The same blocks as struct formats: RotaryArgs; KiviRowsArgs; SharedAttendArgs before and behind its two KiviRowsArgs.
+ROTARY_PACK = struct.Struct("=3Q3Q9q9q3iiqqiiiiQifqqqQ")
+KIVI_ROWS_PACK = struct.Struct("=8Q5q2i")
+SHARED_ATTEND_HEAD = struct.Struct("=4Q8ifi")
+SHARED_ATTEND_TAIL = struct.Struct("=Qq2i")
+
+
 # name -> (restype, argtypes); every symbol include/vqb200.h declares.
 SIGNATURES = {
     "vq_version": (C.c_int32, []),
@@ -232,9 +240,11 @@ SIGNATURES = {
                                          C.c_int32, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),
     "vq_skvq_quantize_pack": (C.c_int32, [C.POINTER(SkvqQuantArgs), C.c_void_p]),
     "vq_skvq_unpack_dequant": (C.c_int32, [C.POINTER(SkvqDequantArgs), C.c_void_p]),
-    "vq_rotary": (C.c_int32, [C.POINTER(RotaryArgs), C.c_void_p]),
-    "vq_kivi_shared_attend_workspace_bytes": (C.c_int64, [C.POINTER(SharedAttendArgs)]),
-    "vq_kivi_shared_attend": (C.c_int32, [C.POINTER(SharedAttendArgs), C.c_void_p]),
+    # (argument blocks passed as packed bytes, see ROTARY_PACK / KIVI_ROWS_PACK / SHARED_ATTEND_*: filling a
+    # Structure field by field costs more than the launch)
+    "vq_rotary": (C.c_int32, [C.c_char_p, C.c_void_p]),
+    "vq_kivi_shared_attend_workspace_bytes": (C.c_int64, [C.c_char_p]),
+    "vq_kivi_shared_attend": (C.c_int32, [C.c_char_p, C.c_void_p]),
     "vq_bit_pack": (C.c_int32, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p]),
     "vq_bit_unpack": (C.c_int32, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p]),
 }

@@ -42,7 +42,7 @@ SOURCES = [
     ("skvq.cu", ["-fmad=false"]),
     ("rotary.cu", []),
     ("shared_attend.cu", []),
-    ("shared_prefix_tc5.cu", []),
+    ("shared_tiles_tc5.cu", []),
 ]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -298,7 +298,7 @@ extern "C" int32_t vq_kivi_attend_status(void) {
     if (rc != VQ_OK) return rc;
     rc = peer_gather_take_timeout(&flag3);
     if (rc != VQ_OK) return rc;
-    rc = shared_prefix_tc5_take_timeout(&flag4);
+    rc = shared_tiles_tc5_take_timeout(&flag4);
     if (rc != VQ_OK) return rc;
     if (flag3) return fail(VQ_ERR_TIMEOUT, "vq_peer_gather_wait: a peer's output rows did not arrive within the poll limit");
     if (flag) return fail(VQ_ERR_TIMEOUT, "vq_kivi_decode_attend: a bounded wait on a bulk-copy barrier gave up");

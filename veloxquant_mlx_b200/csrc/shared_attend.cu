@@ -5,8 +5,8 @@
 //
 // Both parts are attended apart, each split along its tokens, into partial records (m, l, o) that
 // the merge kernel joins: o = sum_j 2^(m_j - M) o_j / sum_j 2^(m_j - M) l_j.
-// The prefix is read once for all B * H_q/H_kv * S_q query rows of a kv head (from 33 rows on by the
-// tcgen05 kernel of shared_prefix_tc5.cu), the own tokens once per request.
+// The prefix is read once for all B * H_q/H_kv * S_q query rows of a kv head, the own tokens once per
+// request. Many query rows go to the tcgen05 kernel of shared_tiles_tc5.cu, few to the warp tiles below.
 #include <algorithm>
 #include <type_traits>
 
@@ -103,6 +103,7 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
     constexpr float BASE = Codes<SB>::kBase;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float sh_m[kWarps][ROWS], sh_l[kWarps][ROWS];
+    let_next_start();
 
     const int lane = threadIdx.x & 31;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
@@ -395,16 +396,17 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
         *reinterpret_cast<float4 *>(p.parts.o + rec * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         if (d == 0) *reinterpret_cast<float2 *>(p.parts.ml + rec * 2) = make_float2(mm, ll);
     }
+    wait_for_previous();  // the merge waits for this kernel alone: it must not end before the tcgen05 kernel does
 }
 
 template <int D, int SB, typename T, int NT>
-int32_t launch_rows(const RowsParams &p, unsigned blocks, cudaStream_t st) {
+int32_t launch_rows(const RowsParams &p, unsigned blocks, bool dependent, cudaStream_t st) {
     constexpr int ring = kWarps * kStages * Stage<D, SB>::BYTES, merge = kWarps * 8 * NT * (D + 4) * 4;
     constexpr int smem = ring > merge ? ring : merge;
-    VQ_CHECK_CUDA(cudaFuncSetAttribute(shared_attend_rows_kernel<D, SB, T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    shared_attend_rows_kernel<D, SB, T, NT><<<blocks, kWarps * 32, smem, st>>>(p);
-    VQ_CHECK_LAUNCH("shared_attend_rows_kernel");
-    return VQ_OK;
+    static std::atomic<uint64_t> allowed{0};
+    const int32_t rc = allow_shared_memory(&shared_attend_rows_kernel<D, SB, T, NT>, smem, allowed);
+    if (rc != VQ_OK) return rc;
+    return launch_dependent(&shared_attend_rows_kernel<D, SB, T, NT>, "shared_attend_rows_kernel", blocks, kWarps * 32, smem, st, dependent, p);
 }
 
 // Joins the records of an output row: `ways` warps (1 or 4) take its records in turn, each lane D/32
@@ -422,6 +424,7 @@ __global__ void __launch_bounds__(128) shared_attend_merge_kernel(const SharedPa
     const int64_t row = (int64_t)blockIdx.x * (4 / ways) + warp / ways;
     const int n = parts.n_splits;
     float ll = 0.f, mm = -INFINITY, acc[C] = {};
+    wait_for_previous();
     if (row < rows) {
         const float2 *ml = reinterpret_cast<const float2 *>(parts.ml) + row * n;
         float2 r[kMaxRecords / 32];
@@ -471,33 +474,37 @@ __global__ void __launch_bounds__(128) shared_attend_merge_kernel(const SharedPa
 }
 
 struct Plan {
-    bool tc5;
-    int row_tile;  // query rows of a warp tile: 8 or 16
-    int np, no;
+    int prefix_tc5, own_tc5;  // splits of the parts that the tcgen05 kernel takes (0: it does not)
+    int np, no;               // partial records of the two parts
+    int row_tile;             // query rows of a warp tile: 8 or 16
     int prefix_tiles, own_tiles;
     int64_t rows;
 };
 
-int groups_of(const vq_kivi_rows &st) { return st.n_quant / kGroup + (st.n_res + kGroup - 1) / kGroup; }
-
 int32_t plan_of(const vq_shared_attend_args &a, const DeviceInfo &di, Plan *out) {
     Plan pl = {};
-    const int64_t per_req = (int64_t)(a.H_q / a.H_kv) * a.S_q;
+    const int64_t per_req = (int64_t)(a.H_q / a.H_kv) * a.S_q, all = a.B * per_req;
     pl.rows = (int64_t)a.B * a.H_q * a.S_q;
-    const int gp = groups_of(a.prefix), go = groups_of(a.own);
-    const int64_t ctas = (int64_t)di.sm_count * 3;
-    auto splits = [&](int64_t units, int groups) {
-        // enough CTAs to fill the GPU, but at least two groups a warp
-        return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(ctas, units), ceil_div(groups, 2 * kWarps), 64}));
-    };
-    const char *why = shared_prefix_tc5_supported(a);
-    VQ_REQUIRE(a.variant != 2 || why == nullptr, VQ_ERR_SHAPE, "vq_kivi_shared_attend: tcgen05 kernel unavailable: %s", why);
-    pl.tc5 = gp > 0 && why == nullptr && a.variant != 1;
-    pl.row_tile = (pl.tc5 ? per_req : a.B * per_req) > 8 ? 16 : 8;
-    pl.prefix_tiles = (int)ceil_div(a.B * per_req, pl.row_tile);
+    const vq_kivi_rows &pre = a.prefix, &own = a.own;
+    const int ip = pre.n_quant / kGroup + (int)ceil_div(pre.n_res, kHalf), io = own.n_quant / kGroup + (int)ceil_div(own.n_res, kHalf);
+    // The tcgen05 kernel decodes a token once for 128 or 256 query rows, the warp tiles for 8 or 16: it
+    // pays from two of the wider ones on (33 rows behind 2K tokens: 12 against 14 us), but not for a prefix
+    // of a few hundred tokens, where its setup shows. It takes scales that are not negative.
+    const bool can = a.scale >= 0.f;
+    VQ_REQUIRE(a.variant != 2 || (can && ip), VQ_ERR_SHAPE, "vq_kivi_shared_attend: the tcgen05 kernel needs a prefix and a scale that is not negative");
+    if (can && ip && (a.variant == 2 || (a.variant == 0 && all > 2 * 16 && (int64_t)pre.n_quant + pre.n_res >= 512)))
+        pl.prefix_tc5 = shared_tiles_tc5_splits(pre, a.H_kv, all, a.n_splits, di);
+    if (can && io && a.variant != 1 && per_req > 2 * 16) pl.own_tc5 = shared_tiles_tc5_splits(own, (int64_t)a.B * a.H_kv, per_req, 0, di);
+    pl.row_tile = (pl.prefix_tc5 ? per_req : all) > 8 ? 16 : 8;
+    pl.prefix_tiles = (int)ceil_div(all, pl.row_tile);
     pl.own_tiles = (int)ceil_div(per_req, pl.row_tile);
-    pl.no = go ? splits((int64_t)a.B * a.H_kv * pl.own_tiles, go) : 0;
-    pl.np = !gp ? 0 : pl.tc5 ? shared_prefix_tc5_splits(a, di) : a.n_splits > 0 ? std::min({a.n_splits, gp, 64}) : splits((int64_t)a.H_kv * pl.prefix_tiles, gp);
+    auto splits = [&](int64_t units, int items) {
+        // enough CTAs to fill the GPU, but at least two work items a warp
+        return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div((int64_t)di.sm_count * 3, units), ceil_div(items, 2 * kWarps), 64}));
+    };
+    pl.np = !ip ? 0 : pl.prefix_tc5 ? shared_tiles_tc5_records(all, pl.prefix_tc5) : a.n_splits > 0 ? std::min({a.n_splits, ip, 64})
+                                                                                                   : splits((int64_t)a.H_kv * pl.prefix_tiles, ip);
+    pl.no = !io ? 0 : pl.own_tc5 ? shared_tiles_tc5_records(per_req, pl.own_tc5) : splits((int64_t)a.B * a.H_kv * pl.own_tiles, io);
     *out = pl;
     return VQ_OK;
 }
@@ -553,27 +560,28 @@ int32_t launch_all(const vq_shared_attend_args &a, const Plan &pl, const DeviceI
     p.parts.ml = p.parts.o + pl.rows * p.parts.n_splits * D;
     p.prefix_tiles = pl.prefix_tiles;
     p.own_tiles = pl.own_tiles;
-    const int64_t pb = pl.tc5 ? 0 : (int64_t)pl.np * pl.prefix_tiles * a.H_kv;
-    const int64_t blocks = pb + (int64_t)pl.no * pl.own_tiles * a.B * a.H_kv;
+    const bool tc5 = pl.prefix_tc5 || pl.own_tc5;
+    const int64_t pb = pl.prefix_tc5 ? 0 : (int64_t)pl.np * pl.prefix_tiles * a.H_kv;
+    const int64_t blocks = pb + (pl.own_tc5 ? 0 : (int64_t)pl.no * pl.own_tiles * a.B * a.H_kv);
     VQ_REQUIRE(blocks < (1ll << 31), VQ_ERR_SHAPE, "vq_kivi_shared_attend: too many query rows for one launch");
     p.prefix_blocks = (int)pb;
-    if (pl.tc5) {
-        const int32_t rc = shared_prefix_tc5_launch(a, p.parts, pl.np, di, st);
+    if (tc5) {
+        const int32_t rc = shared_tiles_tc5_launch(a, p.parts, pl.prefix_tc5, pl.own_tc5, pl.np, st);
         if (rc != VQ_OK) return rc;
     }
     if (blocks) {
+        // (behind the tcgen05 kernel: its blocks fill the SMs as that kernel's finish)
         const bool wide = pl.row_tile == 16;
         const unsigned nb = (unsigned)blocks;
         int32_t rc;
-        if (a.store_bits == 2) rc = wide ? launch_rows<D, 2, T, 2>(p, nb, st) : launch_rows<D, 2, T, 1>(p, nb, st);
-        else if (a.store_bits == 4) rc = wide ? launch_rows<D, 4, T, 2>(p, nb, st) : launch_rows<D, 4, T, 1>(p, nb, st);
-        else rc = wide ? launch_rows<D, 8, T, 2>(p, nb, st) : launch_rows<D, 8, T, 1>(p, nb, st);
+        if (a.store_bits == 2) rc = wide ? launch_rows<D, 2, T, 2>(p, nb, tc5, st) : launch_rows<D, 2, T, 1>(p, nb, tc5, st);
+        else if (a.store_bits == 4) rc = wide ? launch_rows<D, 4, T, 2>(p, nb, tc5, st) : launch_rows<D, 4, T, 1>(p, nb, tc5, st);
+        else rc = wide ? launch_rows<D, 8, T, 2>(p, nb, tc5, st) : launch_rows<D, 8, T, 1>(p, nb, tc5, st);
         if (rc != VQ_OK) return rc;
     }
     const int ways = p.parts.n_splits > 8 ? 4 : 1;
-    shared_attend_merge_kernel<D, T><<<(unsigned)ceil_div(pl.rows * ways, 4), 128, 0, st>>>(p.parts, pl.rows, ways, (T *)a.out, a.lse);
-    VQ_CHECK_LAUNCH("shared_attend_merge_kernel");
-    return VQ_OK;
+    return launch_dependent(&shared_attend_merge_kernel<D, T>, "shared_attend_merge_kernel", (unsigned)ceil_div(pl.rows * ways, 4), 128, 0, st,
+                            tc5 || blocks > 0, p.parts, pl.rows, ways, (T *)a.out, a.lse);
 }
 
 }  // namespace

@@ -1,5 +1,7 @@
 // Internal interface between the shared-prefix attention's entry point and its prefix kernel.
 #pragma once
+#include <atomic>
+
 #include "common.cuh"
 
 namespace vq {
@@ -12,12 +14,48 @@ struct SharedPartials {
     int n_splits;  // prefix splits, then own splits
 };
 
-// Whether the tcgen05 kernel takes the prefix of `a` (NULL) or why not, the splits it would use, its
-// launch into splits [0, np) of `parts`, and its "a bounded wait gave up" flag.
-const char *shared_prefix_tc5_supported(const vq_shared_attend_args &a);
-int shared_prefix_tc5_splits(const vq_shared_attend_args &a, const DeviceInfo &di);
-int32_t shared_prefix_tc5_launch(const vq_shared_attend_args &a, const SharedPartials &parts, int np, const DeviceInfo &di, cudaStream_t st);
-int32_t shared_prefix_tc5_take_timeout(int *flag);
+// The tcgen05 kernel (shared_tiles_tc5.cu): the splits it uses for a store against `units` x `rows` query
+// rows; its launch for the prefix (prefix_splits > 0, records from 0) and the own tokens (own_splits > 0,
+// records from own_record0); its "a bounded wait gave up" flag. A part of at most 128 rows a unit leaves two
+// records per split.
+int shared_tiles_tc5_splits(const vq_kivi_rows &st, int64_t units, int64_t rows, int wanted, const DeviceInfo &di);
+inline int shared_tiles_tc5_records(int64_t rows, int splits) { return rows > 128 ? splits : 2 * splits; }
+int32_t shared_tiles_tc5_launch(const vq_shared_attend_args &a, const SharedPartials &parts, int prefix_splits, int own_splits, int own_record0,
+                                cudaStream_t stream);
+int32_t shared_tiles_tc5_take_timeout(int *flag);
+
+// Opts a kernel into `bytes` of dynamic shared memory, once per device (`done`: one bit a device).
+template <typename K>
+int32_t allow_shared_memory(K *kernel, int bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    VQ_CHECK_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return VQ_OK;
+    VQ_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_release);
+    return VQ_OK;
+}
+
+// Launch as a programmatic dependent of the kernel before it on the stream: its blocks may be placed while
+// that kernel's last blocks finish, and must pass wait_for_previous() before they touch what it writes.
+template <typename... P, typename... A>
+int32_t launch_dependent(void (*kernel)(P...), const char *name, unsigned blocks, int threads, int smem, cudaStream_t st, bool dependent, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = dependent ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+    if (e != cudaSuccess) return fail(VQ_ERR_CUDA, "launch of %s failed: %s", name, cudaGetErrorString(e));
+    return VQ_OK;
+}
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---- packed codes to numbers ------------------------------------------------------------------
 // A code c becomes the float BASE + c by placing its byte into the mantissa of BASE (one byte

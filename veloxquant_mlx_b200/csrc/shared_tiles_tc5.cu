@@ -1,26 +1,27 @@
-// The shared prefix on the fifth-generation tensor cores: all B * H_q/H_kv * S_q query rows of a kv
-// head against ONE copy of its packed keys and values.
+// Shared-prefix attention on the fifth-generation tensor cores: all B * H_q/H_kv * S_q query rows of a
+// kv head against ONE copy of the packed prefix, and, where each request brings many query rows (its own
+// prompt), those rows against the request's own tokens.
 //
 // Per 128 query rows and 128 tokens: S = Q K^T (tcgen05.mma, float16 in, float32 in tensor memory),
 // P = 2^(S scale - m) (float16, back into tensor memory over S), O += P V (A operand from tensor
 // memory). Each CTA keeps two such streams in flight so that the softmax of one runs under the MMAs
 // of the other:
-//   more than 128 rows (TILES = 2): two row tiles share every decoded token tile;
-//   up to 128 rows     (TILES = 1): one row tile, the streams take token tiles in turn and leave two
-//                                   partial records.
+//   more than 128 rows: two row tiles share every decoded token tile;
+//   up to 128 rows:     one row tile, the streams take token tiles in turn and leave two partial records.
 // Roles: warps 0-3 and 4-7 the softmax of stream 0 and 1 (a thread owns a row: no exchange between
 // lanes), warps 8-11 decode keys, 12-15 values, warp 16 issues the MMAs. Codes go from global memory to
-// registers one tile ahead, through one fused multiply-add and one rounding into 128-byte-swizzled
-// operand tiles, two stages each. Decoding once for 128 or 256 rows is what makes dense float16
-// operands affordable (the decode kernel for a few rows folds the scales into its queries instead).
+// registers one tile ahead (a register is refilled as soon as its code is used), through one fused
+// multiply-add and one rounding into 128-byte-swizzled operand tiles, two stages each. Decoding once for
+// 128 or 256 rows is what makes dense float16 operands affordable (the decode kernel for a few rows folds
+// the scales into its queries instead).
 //
-// The reference maximum m of a row moves only when a tile exceeds it by more than 2^8 (weights up to
-// 256 are exact enough in float16 and cannot overflow its sums, which are float32): O in tensor
-// memory is then rescaled by the row's own thread. That S of step i + 1 is complete implies that P V
-// of step i is (MMAs of one thread complete in order), so no further wait is needed.
+// The reference maximum m of a row moves only when 32 scores exceed it by more than 2^8 (weights up to
+// 256 cannot overflow float16, sums are float32): O and the weights already written are then rescaled by
+// the row's own thread. That S of step i + 1 is complete implies that P V of step i is (MMAs of one
+// thread complete in order), so no further wait is needed.
 //
 // Budget of a token tile with two row tiles at 4 bits, in SM clocks: MMAs 2048, exponentials 2048 (16 a
-// clock), instruction issue about 1900, HBM 1040.
+// clock), instruction issue about 2400, HBM 1040.
 //
 // Every wait is bounded; a role that gives up raises a flag (reported by vq_kivi_attend_status), leaves its
 // loop, and the CTA still waits (bounded) for its MMAs and frees its tensor memory.
@@ -156,15 +157,23 @@ __device__ __forceinline__ void scale_p(uint32_t addr, float f) {
     tmem_st8(addr, r);
 }
 
-struct PrefixParams {
-    const void *q;
-    float scale_log2;
-    int B, H_q, H_kv, S_q, G;
+// One of the two parts of a call: the prefix (a unit is a kv head) or the own tokens (a kv head of a request)
+struct Part {
     vq_kivi_rows st;
-    SharedPartials parts;
+    int blocks;       // units x row_blocks x splits
     int splits;       // CTAs along the tokens
-    int row_blocks;   // CTAs along the query rows of a kv head
+    int row_blocks;   // CTAs along the query rows of a unit
+    int rows;         // query rows of a unit
     int tiles_packed, tiles;
+    int record0;      // first partial record
+};
+struct TileParams {
+    const void *q;
+    const int32_t *own_start;
+    float scale_log2;
+    int H_q, H_kv, S_q, G, causal;
+    SharedPartials parts;
+    Part prefix, own;
 };
 
 template <int D>
@@ -173,7 +182,9 @@ struct Layout {
     static constexpr int HALF = kTile * 128;                  // bytes of one half
     static constexpr int TILE = HALVES * HALF;
     static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE;   // two Q tiles, two stages of K and V
-    static constexpr int BARS = 6 * TILE;
+    static constexpr int OUT_ROW = 4 * D + 16;                // a row of O on its way out: padded, conflict-free
+    static constexpr int OUT = 2 * kTile * OUT_ROW;           // (over the tiles, when they are done with)
+    static constexpr int BARS = 6 * TILE > OUT ? 6 * TILE : OUT;
     // padded past half an SM's shared memory: one CTA an SM, as it takes all of tensor memory
     static constexpr int BYTES = BARS + 256 > 120 * 1024 ? BARS + 256 : 120 * 1024;
     // 16-byte chunk `c` (0 .. D/8) of row `r`
@@ -198,8 +209,8 @@ __device__ __forceinline__ uint4 decode8(const uint32_t (&w)[SB == 8 ? 2 : 1], c
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-template <int D, int SB, typename T, int TILES>
-__global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __grid_constant__ PrefixParams p) {
+template <int D, int SB, typename T>
+__global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __grid_constant__ TileParams p) {
     using L = Layout<D>;
     constexpr int CHUNKS = D / 8;      // 8-channel chunks of a row
     constexpr int RB = D * SB / 8;     // bytes of a packed row
@@ -210,78 +221,88 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::BARS + 8 * kBars);
     const uint32_t bar0 = smem_u32(bars);
     auto bar = [&](int i) { return bar0 + 8u * i; };
+    let_next_start();
 
-    int blk = blockIdx.x;
-    const int split = blk % p.splits; blk /= p.splits;
-    const int rb = blk % p.row_blocks;
-    const int hk = blk / p.row_blocks;
-    const int per_req = p.G * p.S_q, n_rows = p.B * per_req;
-    const int row0 = rb * kTile * TILES;
-    const int t_lo = (int)((int64_t)p.tiles * split / p.splits), t_hi = (int)((int64_t)p.tiles * (split + 1) / p.splits);
+    const bool is_prefix = (int)blockIdx.x < p.prefix.blocks;
+    const Part &part = is_prefix ? p.prefix : p.own;
+    int blk = is_prefix ? blockIdx.x : blockIdx.x - p.prefix.blocks;
+    const int split = blk % part.splits; blk /= part.splits;
+    const int rb = blk % part.row_blocks;
+    const int unit = blk / part.row_blocks;
+    const int b_own = is_prefix ? 0 : unit / p.H_kv;
+    const int hk = is_prefix ? unit : unit - b_own * p.H_kv;
+    const int n_rows = part.rows, per_req = p.G * p.S_q;
+    const bool two = n_rows > kTile;                   // two row tiles, or one that both streams work on
+    const int row0 = rb * (two ? 2 * kTile : kTile);
+    const vq_kivi_rows &st = part.st;
+    const int n_slots = st.n_quant + st.n_res, tiles_packed = part.tiles_packed;
+    const int first_slot = is_prefix || !p.own_start ? 0 : min(n_slots, max(0, __ldg(p.own_start + b_own)));
+    const int t_first = first_slot < st.n_quant ? first_slot / kTile : min(part.tiles, tiles_packed + (first_slot - st.n_quant) / kTile);
+    const int t_lo = t_first + (int)((int64_t)(part.tiles - t_first) * split / part.splits);
+    const int t_hi = t_first + (int)((int64_t)(part.tiles - t_first) * (split + 1) / part.splits);
     const int n_tiles = t_hi - t_lo;
-    const int n_steps = TILES == 2 ? 2 * n_tiles : n_tiles;
-    const vq_kivi_rows &st = p.st;
+    const int n_steps = two ? 2 * n_tiles : n_tiles;
 
-    auto out_row = [&](int r) {  // output row (= row of q) of this kv head's query row r
-        const int b = r / per_req;
-        return ((int64_t)b * p.H_q + (int64_t)hk * p.G) * p.S_q + (r - b * per_req);
+    auto out_row = [&](int r) {  // output row (= row of q) of the unit's query row r
+        const int b = is_prefix ? r / per_req : b_own, rem = is_prefix ? r - b * per_req : r;
+        return ((int64_t)b * p.H_q + (int64_t)hk * p.G) * p.S_q + rem;
+    };
+    bool gave_up = false;
+    auto wait = [&](int b, uint32_t parity) {  // by whole warps: all lanes go on or none
+        if (!gave_up) gave_up = !__all_sync(0xffffffffu, mbar_wait(bar(b), parity));
+        return !gave_up;
+    };
+    uint32_t tmem = 0;
+    // Everything before the roles' loops: what the loops need is complete and visible behind it. The
+    // decoding warps ask for their first codes before they come here.
+    auto ready = [&]() {
+        fence_async_smem();
+        fence_before();
+        __syncthreads();
+        fence_after();
+        tmem = *tmem_slot;
     };
 
     if ((smem_u32(smem) & 1023u) != 0) {  // the swizzle assumes it; never seen
         if (tid == 0) atomicExch(&g_shared_timeout, 2);
         return;
     }
-    if (tid == 0) {
-        for (int i = 0; i < kBars; ++i) {
-            const bool by_warps = i < kKEmpty || (i >= kVFull && i < kVEmpty) || (i >= kPReady && i < kODone);
-            mbar_init(bar(i), by_warps ? 4 : 1);
-        }
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == 16) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    // the query tiles, as halves; rows behind the last are zero
-    for (int i = tid; i < TILES * kTile * CHUNKS; i += kThreads) {
-        const int r = i / CHUNKS, c = i % CHUNKS;
-        uint4 v = zero4();
-        if (row0 + r < n_rows) {
-            v = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(p.q) + out_row(row0 + r) * D) + c);
-            v = make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w));
-        }
-        *reinterpret_cast<uint4 *>(smem + L::Q + (r / kTile) * L::TILE + L::at(r % kTile, c)) = v;
-    }
-    fence_async_smem();
-    fence_before();
-    __syncthreads();
-    fence_after();
-    const uint32_t tmem = *tmem_slot;
-    // scores (and the weights over them) of stream s: columns 128 s; its output: 256 + 128 s
-    bool gave_up = false;
-    auto wait = [&](int b, uint32_t parity) {  // by whole warps: all lanes go on or none
-        if (!gave_up) gave_up = !__all_sync(0xffffffffu, mbar_wait(bar(b), parity));
-        return !gave_up;
-    };
-
+    // scores (and the weights over them) of stream s: columns 128 s of tensor memory; its output: 256 + 128 s
     if (warp < 8) {
         // ---- softmax: thread = row -----------------------------------------------------------------
+        // first the query tiles, as halves; rows behind the last are zero
+        for (int i = tid; i < (two ? 2 : 1) * kTile * CHUNKS; i += 256) {
+            const int r = i / CHUNKS, c = i % CHUNKS;
+            uint4 v = zero4();
+            if (row0 + r < n_rows) {
+                v = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(p.q) + out_row(row0 + r) * D) + c);
+                v = make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w));
+            }
+            *reinterpret_cast<uint4 *>(smem + L::Q + (r / kTile) * L::TILE + L::at(r % kTile, c)) = v;
+        }
+        ready();
         const int s = warp >> 2;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + 128 * s + lane_base, to = ts + 256;
-        const int n_mine = TILES == 2 ? n_tiles : (n_tiles - s + 1) / 2;
+        const int n_mine = two ? n_tiles : (n_tiles - s + 1) / 2;
+        const int r = row0 + (two ? s * kTile : 0) + (warp & 3) * 32 + lane;
+        // slots [first_slot, lim) are seen by this row
+        const int lim = is_prefix || !p.causal ? n_slots : n_slots - p.S_q + r % p.S_q + 1;
         float m = -INFINITY, l = 0.f;  // reference maximum (times scale, base 2) and the weights' sum
         for (int i = 0; i < n_mine; ++i) {
-            const int t = t_lo + (TILES == 2 ? i : 2 * i + s);
-            const int nv = t < p.tiles_packed ? min(kTile, st.n_quant - t * kTile) : min(kTile, st.n_res - (t - p.tiles_packed) * kTile);
+            const int t = t_lo + (two ? i : 2 * i + s);
+            const int slot0 = t < tiles_packed ? t * kTile : st.n_quant + (t - tiles_packed) * kTile;
+            // columns [lo, hi) of the tile
+            const int lo = first_slot - slot0, hi = min(lim, t < tiles_packed ? st.n_quant : n_slots) - slot0;
+            const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < kTile);
             if (!wait(kSFull + s, i & 1)) break;
             fence_after();
             float2 sum[2] = {};
             // 32 scores (already loaded) to weights; their largest may first raise m
             auto chunk = [&](int c, float (&v)[32]) {
-                if (nv < c + 32) {
+                if (masked) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] = c + k < nv ? v[k] : -INFINITY;
+                    for (int k = 0; k < 32; ++k) v[k] = c + k >= lo && c + k < hi ? v[k] : -INFINITY;
                 }
                 float mx = max3(v[0], v[1], v[2]), m1 = max3(v[3], v[4], v[5]);
 #pragma unroll
@@ -333,24 +354,30 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kPReady + s));
         }
-        if (n_mine > 0) wait(kODone + s, 0);
+        // O goes out through shared memory: a row a lane there, whole rows at a time to global memory. The
+        // tiles it overwrites are done with when both streams are.
+        if (n_steps > 0) wait(kODone, 0);
+        if (n_steps > 1) wait(kODone + 1, 0);
         fence_after();
-        const int r = row0 + (TILES == 2 ? s * kTile : 0) + (warp & 3) * 32 + lane;
         const bool live = r < n_rows;
-        const int64_t rec = live ? out_row(r) * p.parts.n_splits + (TILES == 2 ? split : 2 * split + s) : 0;
+        const int64_t rec = live ? out_row(r) * p.parts.n_splits + part.record0 + (two ? split : 2 * split + s) : 0;
+        uint8_t *mine = smem + (warp * 32 + lane) * L::OUT_ROW;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = 0; c < D; c += 32) {
             float v[32];
-            tmem_ld32(to + 32 * c, v);
+            tmem_ld32(to + c, v);
             tmem_ld_wait(v);
-            if (live) {
 #pragma unroll
-                for (int k = 0; k < 32; k += 4)
-                    *reinterpret_cast<float4 *>(p.parts.o + rec * D + 32 * c + k) =
-                        n_mine > 0 ? make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
+            for (int k = 0; k < 32; k += 4)
+                *reinterpret_cast<float4 *>(mine + 4 * (c + k)) = n_mine > 0 ? make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        if (live) *reinterpret_cast<float2 *>(p.parts.ml + rec * 2) = make_float2(m, l);
+        fence_async_smem();
+        if (live) {
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.parts.o + rec * D), "r"(smem_u32(mine)), "n"(4 * D) : "memory");
+            *reinterpret_cast<float2 *>(p.parts.ml + rec * 2) = make_float2(m, l);
+        }
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     } else if (warp < 12) {
         // ---- keys: warp w decodes the w-th 32-token group of a tile -----------------------------------
         // lane = (token parity, chunk of 8 channels): the group's scales and zeros of 8 channels stay in registers
@@ -358,12 +385,12 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
         constexpr int N = kGroup / TPL;           // tokens a lane decodes
         constexpr int W = SB == 8 ? 2 : 1;
         const int w = warp - 8, chunk = lane % CHUNKS, sub = lane / CHUNKS;
-        const uint8_t *codes = st.k_codes + hk * st.k_codes_stride_bh;
-        const float *ks = st.k_scale + hk * st.k_param_stride_bh, *kz = st.k_zero + hk * st.k_param_stride_bh;
-        const T *exact = reinterpret_cast<const T *>(st.k_res) + hk * st.res_stride_bh;
+        const uint8_t *codes = st.k_codes + unit * st.k_codes_stride_bh;
+        const float *ks = st.k_scale + unit * st.k_param_stride_bh, *kz = st.k_zero + unit * st.k_param_stride_bh;
+        const T *exact = reinterpret_cast<const T *>(st.k_res) + unit * st.res_stride_bh;
         uint32_t cur[N][W];   // codes of the tile to decode; each is replaced by the next tile's once it is used
         float4 ns[2], nz[2];  // its scales and zeros
-        auto here = [&](int t) { return t < min(t_hi, p.tiles_packed) && t * kTile + w * kGroup < st.n_quant; };
+        auto here = [&](int t) { return t < min(t_hi, tiles_packed) && t * kTile + w * kGroup < st.n_quant; };
         auto fetch_codes = [&](int t, int i) {
             const uint8_t *src = codes + ((int64_t)t * kTile + w * kGroup + TPL * i + sub) * RB + chunk * SB;
             if constexpr (SB == 8) {
@@ -383,10 +410,20 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
 #pragma unroll
             for (int i = 0; i < N; ++i) fetch_codes(t_lo, i);
         }
+        // (token k of this lane is row 32 w + TPL k + sub: its chunk's place turns with the row modulo 8)
+        const uint32_t at0 = L::at(w * kGroup + sub, chunk);
+        auto place = [&](int stage, int k) { return smem + L::K + stage * L::TILE + ((at0 ^ ((TPL * k & 7) << 4)) + TPL * k * 128); };
+        if (warp == 8 && elect_one()) {
+            for (int i = 0; i < kBars; ++i) {
+                const bool by_warps = i < kKEmpty || (i >= kVFull && i < kVEmpty) || (i >= kPReady && i < kODone);
+                mbar_init(bar(i), by_warps ? 4 : 1);
+            }
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        ready();
         for (int i = 0; i < n_tiles; ++i) {
             const int t = t_lo + i, stage = i & 1;
-            uint8_t *dst = smem + L::K + stage * L::TILE;
-            if (t < p.tiles_packed) {
+            if (t < tiles_packed) {
                 const bool some = here(t), more = here(t + 1);
                 const float2 sc[4] = {{ns[0].x, ns[0].y}, {ns[0].z, ns[0].w}, {ns[1].x, ns[1].y}, {ns[1].z, ns[1].w}};
                 const float2 zz[4] = {{nz[0].x, nz[0].y}, {nz[0].z, nz[0].w}, {nz[1].x, nz[1].y}, {nz[1].z, nz[1].w}};
@@ -398,16 +435,16 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
                 if (some) {
 #pragma unroll
                     for (int k = 0; k < N; ++k) {
-                        *reinterpret_cast<uint4 *>(dst + L::at(w * kGroup + TPL * k + sub, chunk)) = decode8<SB>(cur[k], sc, ze);
+                        *reinterpret_cast<uint4 *>(place(stage, k)) = decode8<SB>(cur[k], sc, ze);
                         if (more) fetch_codes(t + 1, k);
                     }
                 } else {
 #pragma unroll 1
-                    for (int k = 0; k < N; ++k) *reinterpret_cast<uint4 *>(dst + L::at(w * kGroup + TPL * k + sub, chunk)) = zero4();
+                    for (int k = 0; k < N; ++k) *reinterpret_cast<uint4 *>(place(stage, k)) = zero4();
                 }
             } else {
                 if (i >= 2 && !wait(kKEmpty + stage, ((i >> 1) - 1) & 1)) break;
-                const int r0 = (t - p.tiles_packed) * kTile + w * kGroup;
+                const int r0 = (t - tiles_packed) * kTile + w * kGroup;
 #pragma unroll 2
                 for (int k = 0; k < N; ++k) {
                     const int row = r0 + TPL * k + sub;
@@ -416,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
                         v = __ldg(reinterpret_cast<const uint4 *>(exact + (int64_t)row * D) + chunk);
                         v = make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w));
                     }
-                    *reinterpret_cast<uint4 *>(dst + L::at(w * kGroup + TPL * k + sub, chunk)) = v;
+                    *reinterpret_cast<uint4 *>(place(stage, k)) = v;
                 }
             }
             fence_async_smem();
@@ -430,12 +467,12 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
         constexpr int N = kTile / TPI;            // tokens a thread decodes
         constexpr int W = SB;                     // words of 32 codes
         const int vt = tid - 12 * 32, grp = vt % GV, tok = vt / GV;
-        const uint8_t *codes = st.v_codes + hk * st.v_codes_stride_bh;
-        const float *vs = st.v_scale + hk * st.v_param_stride_bh, *vz = st.v_zero + hk * st.v_param_stride_bh;
-        const T *exact = reinterpret_cast<const T *>(st.v_res) + hk * st.res_stride_bh;
+        const uint8_t *codes = st.v_codes + unit * st.v_codes_stride_bh;
+        const float *vs = st.v_scale + unit * st.v_param_stride_bh, *vz = st.v_zero + unit * st.v_param_stride_bh;
+        const T *exact = reinterpret_cast<const T *>(st.v_res) + unit * st.res_stride_bh;
         uint32_t cur[N][W];   // as for the keys
         float sc[N], ze[N];
-        auto here = [&](int t, int i) { return t < min(t_hi, p.tiles_packed) && t * kTile + i * TPI + tok < st.n_quant; };
+        auto here = [&](int t, int i) { return t < min(t_hi, tiles_packed) && t * kTile + i * TPI + tok < st.n_quant; };
         auto fetch = [&](int t, int i) {
             const int64_t slot = (int64_t)t * kTile + i * TPI + tok;
             const uint8_t *src = codes + slot * RB + grp * (4 * SB);
@@ -455,15 +492,18 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (here(t_lo, i)) fetch(t_lo, i);
+        // (row k TPI + tok, chunk 4 grp + j: TPI is a multiple of 8, so only j moves the place)
+        const uint32_t at0 = L::at(tok, 4 * grp);
+        auto place = [&](int stage, int k, int j) { return smem + L::V + stage * L::TILE + ((at0 ^ (j << 4)) + k * TPI * 128); };
+        ready();
         for (int i = 0; i < n_tiles; ++i) {
             const int t = t_lo + i, stage = i & 1;
-            uint8_t *dst = smem + L::V + stage * L::TILE;
-            if (t < p.tiles_packed) {
+            if (t < tiles_packed) {
                 if (i >= 2 && !wait(kVEmpty + stage, ((i >> 1) - 1) & 1)) break;
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
-                    const int row = k * TPI + tok;
-                    const bool some = here(t, k);
+                    // (values of padding must not reach P V, where their weight is 0, as infinity or NaN)
+                    const bool some = here(t, k) && t * kTile + k * TPI + tok >= first_slot;
                     const float sk = sc[k], zk = fmaf(-Codes<SB>::kBase, sc[k], ze[k]);
                     const float2 s8[4] = {{sk, sk}, {sk, sk}, {sk, sk}, {sk, sk}}, z8[4] = {{zk, zk}, {zk, zk}, {zk, zk}, {zk, zk}};
 #pragma unroll
@@ -472,24 +512,24 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
                         if constexpr (SB == 8) { wd[0] = cur[k][2 * j]; wd[1] = cur[k][2 * j + 1]; }
                         else if constexpr (SB == 4) wd[0] = cur[k][j];
                         else wd[0] = cur[k][j / 2] >> (16 * (j & 1));
-                        *reinterpret_cast<uint4 *>(dst + L::at(row, 4 * grp + j)) = some ? decode8<SB>(wd, s8, z8) : zero4();
+                        *reinterpret_cast<uint4 *>(place(stage, k, j)) = some ? decode8<SB>(wd, s8, z8) : zero4();
                     }
                     if (here(t + 1, k)) fetch(t + 1, k);
                 }
             } else {
                 if (i >= 2 && !wait(kVEmpty + stage, ((i >> 1) - 1) & 1)) break;
-                const int r0 = (t - p.tiles_packed) * kTile;
+                const int r0 = (t - tiles_packed) * kTile;
 #pragma unroll 1
                 for (int k = 0; k < N; ++k) {
                     const int row = k * TPI + tok;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint4 v = zero4();
-                        if (r0 + row < st.n_res) {
+                        if (r0 + row < st.n_res && st.n_quant + r0 + row >= first_slot) {
                             v = __ldg(reinterpret_cast<const uint4 *>(exact + (int64_t)(r0 + row) * D) + 4 * grp + j);
                             v = make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w));
                         }
-                        *reinterpret_cast<uint4 *>(dst + L::at(row, 4 * grp + j)) = v;
+                        *reinterpret_cast<uint4 *>(place(stage, k, j)) = v;
                     }
                 }
             }
@@ -501,14 +541,17 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
         // ---- the MMAs, all by one thread, in order ------------------------------------------------------
         // (the whole warp walks through the loop, so that descriptors stay in uniform registers)
         const bool elected = elect_one();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        ready();
         // (a descriptor's low word holds the address in 16-byte units: stages and k-steps are added to it)
         const uint64_t dq = make_desc(smem_u32(smem + L::Q), 16, 1024), dk = make_desc(smem_u32(smem + L::K), 16, 1024);
         const uint64_t dv = make_desc(smem_u32(smem + L::V), L::HALF, 1024);
         auto qk = [&](int j) {
-            const int s = j & 1, t = TILES == 2 ? j >> 1 : j, stage = t & 1;
-            if ((TILES == 1 || s == 0) && !wait(kKFull + stage, (t >> 1) & 1)) return;
+            const int s = j & 1, t = two ? j >> 1 : j, stage = t & 1;
+            if ((!two || s == 0) && !wait(kKFull + stage, (t >> 1) & 1)) return;
             fence_after();
-            const uint64_t a = dq + (TILES == 2 ? s * (L::TILE >> 4) : 0), b = dk + stage * (L::TILE >> 4);
+            const uint64_t a = dq + (two ? s * (L::TILE >> 4) : 0), b = dk + stage * (L::TILE >> 4);
             const uint32_t d = tmem + 128 * s;
             if (elected) {
 #pragma unroll
@@ -517,13 +560,13 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
                     mma_ss(d, a + off, b + off, make_idesc(kTile, false), k > 0);
                 }
                 mma_commit(bar(kSFull + s));
-                if (TILES == 1 || s == 1) mma_commit(bar(kKEmpty + stage));
+                if (!two || s == 1) mma_commit(bar(kKEmpty + stage));
             }
             __syncwarp();
         };
         auto pv = [&](int j) {
-            const int s = j & 1, t = TILES == 2 ? j >> 1 : j, stage = t & 1;
-            if ((TILES == 1 || s == 0) && !wait(kVFull + stage, (t >> 1) & 1)) return;
+            const int s = j & 1, t = two ? j >> 1 : j, stage = t & 1;
+            if ((!two || s == 0) && !wait(kVFull + stage, (t >> 1) & 1)) return;
             if (!wait(kPReady + s, (j >> 1) & 1)) return;
             fence_after();
             const uint64_t b = dv + stage * (L::TILE >> 4);
@@ -531,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
             if (elected) {
 #pragma unroll
                 for (int k = 0; k < kTile / 16; ++k) mma_ts(d, a + 8 * k, b + k * (2048 >> 4), make_idesc(D, true), j >= 2 || k > 0);
-                if (TILES == 1 || s == 1) mma_commit(bar(kVEmpty + stage));
+                if (!two || s == 1) mma_commit(bar(kVEmpty + stage));
                 if (j + 2 >= n_steps) mma_commit(bar(kODone + s));
             }
             __syncwarp();
@@ -556,79 +599,77 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc5_kernel(const __
     }
 }
 
-int64_t rows_of(const vq_shared_attend_args &a) { return (int64_t)a.B * (a.H_q / a.H_kv) * a.S_q; }
-int tiles_of(const vq_shared_attend_args &a) { return (int)(ceil_div(a.prefix.n_quant, kTile) + ceil_div(a.prefix.n_res, kTile)); }
-int row_tiles(const vq_shared_attend_args &a) { return rows_of(a) > kTile ? 2 : 1; }
+int tiles_of(const vq_kivi_rows &st) { return (int)(ceil_div(st.n_quant, kTile) + ceil_div(st.n_res, kTile)); }
+int row_blocks_of(int64_t rows) { return (int)ceil_div(rows, rows > kTile ? 2 * kTile : kTile); }
 
-template <int D, int SB, typename T, int TILES>
-int32_t launch(const PrefixParams &p, unsigned blocks, cudaStream_t st) {
-    VQ_CHECK_CUDA(cudaFuncSetAttribute(shared_prefix_tc5_kernel<D, SB, T, TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::BYTES));
-    shared_prefix_tc5_kernel<D, SB, T, TILES><<<blocks, kThreads, Layout<D>::BYTES, st>>>(p);
-    VQ_CHECK_LAUNCH("shared_prefix_tc5_kernel");
+template <int D, int SB, typename T>
+int32_t launch(const TileParams &p, unsigned blocks, cudaStream_t st) {
+    static std::atomic<uint64_t> allowed{0};
+    const int32_t rc = allow_shared_memory(&shared_tiles_tc5_kernel<D, SB, T>, Layout<D>::BYTES, allowed);
+    if (rc != VQ_OK) return rc;
+    shared_tiles_tc5_kernel<D, SB, T><<<blocks, kThreads, Layout<D>::BYTES, st>>>(p);
+    VQ_CHECK_LAUNCH("shared_tiles_tc5_kernel");
     return VQ_OK;
 }
-template <int D, int SB, typename T>
-int32_t launch_rows(const PrefixParams &p, int tiles, unsigned blocks, cudaStream_t st) {
-    return tiles == 2 ? launch<D, SB, T, 2>(p, blocks, st) : launch<D, SB, T, 1>(p, blocks, st);
-}
 template <int D, typename T>
-int32_t launch_bits(int sb, const PrefixParams &p, int tiles, unsigned blocks, cudaStream_t st) {
-    if (sb == 2) return launch_rows<D, 2, T>(p, tiles, blocks, st);
-    if (sb == 4) return launch_rows<D, 4, T>(p, tiles, blocks, st);
-    return launch_rows<D, 8, T>(p, tiles, blocks, st);
+int32_t launch_bits(int sb, const TileParams &p, unsigned blocks, cudaStream_t st) {
+    if (sb == 2) return launch<D, 2, T>(p, blocks, st);
+    if (sb == 4) return launch<D, 4, T>(p, blocks, st);
+    return launch<D, 8, T>(p, blocks, st);
 }
 
 }  // namespace
 
-const char *shared_prefix_tc5_supported(const vq_shared_attend_args &a) {
-    if (!(a.scale >= 0.f)) return "the scale must not be negative";
-    if (a.prefix.n_quant + a.prefix.n_res == 0) return "the prefix is empty";
-    // up to two warp tiles of 16 rows decode a token no more often than this kernel's setup costs
-    if (a.variant != 2 && (rows_of(a) <= 32 || tiles_of(a) < 4)) return "few query rows or tokens";
-    return nullptr;
-}
-
-// Partial records of the prefix: one per split, two where the streams share a row tile.
-int shared_prefix_tc5_splits(const vq_shared_attend_args &a, const DeviceInfo &di) {
-    const int tiles = tiles_of(a), rt = row_tiles(a);
-    const int64_t units = (int64_t)a.H_kv * ceil_div(rows_of(a), kTile * rt);
+// Splits of one part along its tokens. The time of a split count, in token tiles: waves of CTAs (one an
+// SM) times the longest CTA (its tiles and a fixed part for setup and epilogue), plus the merge's
+// reading of the records.
+int shared_tiles_tc5_splits(const vq_kivi_rows &st, int64_t units, int64_t rows, int wanted, const DeviceInfo &di) {
+    const int tiles = tiles_of(st), most = std::min(tiles, 32);
+    if (wanted > 0) return std::min(wanted, most);
+    const int64_t ctas = units * row_blocks_of(rows);
+    const int rt = rows > kTile ? 2 : 1;
     int best = 1;
-    if (a.n_splits > 0) {
-        best = std::min({a.n_splits, tiles, 32});
-    } else {
-        // The time of a split count, in token tiles: waves of CTAs (one an SM) times the longest CTA (its
-        // tiles and a fixed part for setup and epilogue), plus the merge's reading of the records.
-        double cheapest = 1e30;
-        for (int s = 1; s <= std::min(tiles, 32); ++s) {
-            const double waves = (double)ceil_div(units * s, di.sm_count);
-            const double t = waves * ((double)ceil_div(tiles, s) + 3.0) + 0.02 * s * (double)ceil_div(units * rt * s, di.sm_count);
-            if (t < cheapest) { cheapest = t; best = s; }
-        }
+    double cheapest = 1e30;
+    for (int s = 1; s <= most; ++s) {
+        const double waves = (double)ceil_div(ctas * s, di.sm_count);
+        const double t = waves * ((double)ceil_div(tiles, s) + 3.0) + 0.02 * s * (double)ceil_div(ctas * rt * s, di.sm_count);
+        if (t < cheapest) { cheapest = t; best = s; }
     }
-    return rt == 1 ? 2 * best : best;
+    return best;
 }
 
-int32_t shared_prefix_tc5_launch(const vq_shared_attend_args &a, const SharedPartials &parts, int np, const DeviceInfo &di, cudaStream_t st) {
-    (void)di;
-    const int rt = row_tiles(a);
-    PrefixParams p = {};
+int32_t shared_tiles_tc5_launch(const vq_shared_attend_args &a, const SharedPartials &parts, int prefix_splits, int own_splits, int own_record0,
+                                cudaStream_t stream) {
+    const int64_t per_req = (int64_t)(a.H_q / a.H_kv) * a.S_q;
+    TileParams p = {};
     p.q = a.q;
+    p.own_start = a.own_start;
     p.scale_log2 = a.scale * 1.4426950408889634f;
-    p.B = a.B; p.H_q = a.H_q; p.H_kv = a.H_kv; p.S_q = a.S_q; p.G = a.H_q / a.H_kv;
-    p.st = a.prefix;
+    p.H_q = a.H_q; p.H_kv = a.H_kv; p.S_q = a.S_q; p.G = a.H_q / a.H_kv;
+    p.causal = (a.flags & VQ_ATTEND_CAUSAL) != 0;
     p.parts = parts;
-    p.splits = rt == 1 ? np / 2 : np;
-    p.row_blocks = (int)ceil_div(rows_of(a), kTile * rt);
-    p.tiles_packed = (int)ceil_div(a.prefix.n_quant, kTile);
-    p.tiles = tiles_of(a);
-    const int64_t blocks = (int64_t)p.splits * p.row_blocks * a.H_kv;
+    int64_t blocks = 0;
+    auto part = [&](Part &t, const vq_kivi_rows &st, int64_t units, int64_t rows, int splits, int record0) {
+        t.st = st;
+        t.splits = std::max(splits, 1);
+        t.rows = (int)rows;
+        t.row_blocks = row_blocks_of(rows);
+        t.tiles_packed = (int)ceil_div(st.n_quant, kTile);
+        t.tiles = tiles_of(st);
+        t.record0 = record0;
+        const int64_t n = splits > 0 ? units * t.row_blocks * splits : 0;
+        t.blocks = (int)std::min<int64_t>(n, INT32_MAX);
+        blocks += n;
+    };
+    part(p.prefix, a.prefix, a.H_kv, a.B * per_req, prefix_splits, 0);
+    part(p.own, a.own, (int64_t)a.B * a.H_kv, per_req, own_splits, own_record0);
     VQ_REQUIRE(blocks < (1ll << 31), VQ_ERR_SHAPE, "vq_kivi_shared_attend: too many query rows for one launch");
     const unsigned nb = (unsigned)blocks;
-    if (a.dtype == VQ_F16) return a.D == 128 ? launch_bits<128, __half>(a.store_bits, p, rt, nb, st) : launch_bits<64, __half>(a.store_bits, p, rt, nb, st);
-    return a.D == 128 ? launch_bits<128, __nv_bfloat16>(a.store_bits, p, rt, nb, st) : launch_bits<64, __nv_bfloat16>(a.store_bits, p, rt, nb, st);
+    if (a.dtype == VQ_F16) return a.D == 128 ? launch_bits<128, __half>(a.store_bits, p, nb, stream) : launch_bits<64, __half>(a.store_bits, p, nb, stream);
+    return a.D == 128 ? launch_bits<128, __nv_bfloat16>(a.store_bits, p, nb, stream) : launch_bits<64, __nv_bfloat16>(a.store_bits, p, nb, stream);
 }
 
-int32_t shared_prefix_tc5_take_timeout(int *flag) {
+int32_t shared_tiles_tc5_take_timeout(int *flag) {
     VQ_CHECK_CUDA(cudaDeviceSynchronize());
     const int zero = 0;
     VQ_CHECK_CUDA(cudaMemcpyFromSymbol(flag, g_shared_timeout, sizeof(int)));

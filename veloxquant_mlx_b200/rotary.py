@@ -17,9 +17,10 @@ from typing import Any
 import torch
 
 from . import _lib
-from ._lib import RotaryArgs, check, dtype_code, lib, require_cuda, stream_ptr
+from ._lib import ROTARY_PACK, check, dtype_code, lib, require_cuda, stream_ptr
 
 _LAYOUTS = ("half", "interleaved")
+_NONE = (0, 0, 0, 0)
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
@@ -126,6 +127,7 @@ class RotaryEmbedding:
             if tuple(freq.shape) != (rotary_dim // 2,):
                 raise ValueError(f"RotaryEmbedding: inv_freq must have shape ({rotary_dim // 2},), got {tuple(freq.shape)}")
         self.head_dim, self.rotary_dim, self.layout = int(head_dim), rotary_dim, layout
+        self._layout_code = _LAYOUTS.index(layout)
         self.inv_freq = freq
         self.attention_factor = float(factor if attention_factor is None else attention_factor)
         self._turns_host = freq / (2.0 * math.pi)
@@ -148,15 +150,18 @@ class RotaryEmbedding:
 
     # -- checks --------------------------------------------------------------------------
     def _check(self, fn, q, k):
-        for name, t in (("q", q), ("k", k)):
-            if t is None:
-                continue
-            if t.ndim != 4 or t.shape[3] != self.head_dim:
-                raise ValueError(f"{fn}: {name} must be [B, H, S, {self.head_dim}], got {tuple(t.shape)}")
-            if t.dtype not in _DTYPES:
-                raise ValueError(f"{fn}: unsupported dtype {t.dtype}; expected float16, bfloat16 or float32")
-        if k is not None and (k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.dtype is not q.dtype or k.device != q.device):
-            raise ValueError(f"{fn}: q {tuple(q.shape)} {q.dtype} on {q.device} and k {tuple(k.shape)} {k.dtype} on {k.device} must agree in "
+        shape, dt = q.shape, q.dtype
+        if len(shape) != 4 or shape[3] != self.head_dim:
+            raise ValueError(f"{fn}: q must be [B, H, S, {self.head_dim}], got {tuple(shape)}")
+        if dt not in _DTYPES:
+            raise ValueError(f"{fn}: unsupported dtype {dt}; expected float16, bfloat16 or float32")
+        if k is None:
+            return
+        ks = k.shape
+        if len(ks) != 4 or ks[3] != self.head_dim:
+            raise ValueError(f"{fn}: k must be [B, H, S, {self.head_dim}], got {tuple(ks)}")
+        if ks[0] != shape[0] or ks[2] != shape[2] or k.dtype is not dt or k.device != q.device:
+            raise ValueError(f"{fn}: q {tuple(shape)} {dt} on {q.device} and k {tuple(ks)} {k.dtype} on {k.device} must agree in "
                              "batch, tokens, dtype and device")
 
     def _check_append(self, q, k, v):
@@ -174,35 +179,36 @@ class RotaryEmbedding:
             return None, 0, 0, 0
         if isinstance(positions, int):
             return None, 0, 0, positions
-        if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
+        if not isinstance(positions, torch.Tensor) or (positions.dtype is not torch.int64 and positions.dtype is not torch.int32):
             raise ValueError(f"{fn}: positions must be an int or an int32 / int64 tensor")
-        shape = tuple(positions.shape)
-        if shape not in ((S,), (1, S), (B, S)):
+        shape, st = positions.shape, positions.stride()
+        if len(shape) == 2 and shape[1] == S and (shape[0] == B or shape[0] == 1):
+            sb = st[0] if shape[0] > 1 else 0
+        elif len(shape) == 1 and shape[0] == S:
+            sb = 0
+        else:
             raise ValueError(f"{fn}: positions must be [{S}], [1, {S}] or [{B}, {S}], got {list(shape)}")
         if positions.device != device:
             raise ValueError(f"{fn}: positions are on {positions.device}, q on {device}")
-        st = positions.stride()
-        return positions, (st[0] if len(shape) == 2 and shape[0] == B and B > 1 else 0), st[-1], 0
+        return positions, sb, st[-1], 0
 
-    def _launch(self, fn, B, S, dtype, device, tensors, positions, inverse) -> None:
-        """``tensors``: up to three ``(input, output or (address, strides))``; the third is copied."""
-        pos, psb, pss, off = self._positions(fn, positions, B, S, device)
-        a = RotaryArgs(dtype=dtype_code(dtype), B=B, S=S, D=self.head_dim, rotary_dim=self.rotary_dim,
-                       layout=1 if self.layout == "interleaved" else 0, inverse=1 if inverse else 0,
-                       positions=None if pos is None else pos.data_ptr(), pos_bytes=8 if pos is None else pos.element_size(),
-                       factor=self.attention_factor, pos_stride_b=psb, pos_stride_s=pss, pos_offset=off, turns=self._turns_on(device))
-        xs, ys = a.x_stride, a.y_stride
-        for i, (x, y) in enumerate(tensors):
-            a.x[i] = x.data_ptr()
-            a.heads[i] = x.shape[1]
-            xs[3 * i], xs[3 * i + 1], xs[3 * i + 2], _ = x.stride()
-            if isinstance(y, torch.Tensor):
-                a.y[i] = y.data_ptr()
-                ys[3 * i], ys[3 * i + 1], ys[3 * i + 2], _ = y.stride()
-            else:
-                a.y[i], (ys[3 * i], ys[3 * i + 1], ys[3 * i + 2], _) = y
-        with _lib.on_device(device):
-            check(lib().vq_rotary(a, stream_ptr(device)), fn)
+    def _launch(self, fn, q, q_out, k, k_out, k_out_stride, v, v_out, v_out_stride, positions, inverse) -> None:
+        """``q`` to the tensor ``q_out``; ``k`` turned and ``v`` copied to addresses (or None)."""
+        B, Hq, S, D = q.shape
+        dev = q.device
+        pos, psb, pss, off = self._positions(fn, positions, B, S, dev)
+        x0, x1, x2, _ = q.stride()
+        y0, y1, y2, _ = q_out.stride()
+        k0, k1, k2, _ = k.stride() if k is not None else _NONE
+        v0, v1, v2, _ = v.stride() if v is not None else _NONE
+        a = ROTARY_PACK.pack(
+            q.data_ptr(), 0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(), q_out.data_ptr(), k_out, v_out,
+            x0, x1, x2, k0, k1, k2, v0, v1, v2, y0, y1, y2, *k_out_stride, *v_out_stride,
+            Hq, 0 if k is None else k.shape[1], 0 if v is None else v.shape[1], dtype_code(q.dtype), B, S, D, self.rotary_dim,
+            self._layout_code, 1 if inverse else 0, 0 if pos is None else pos.data_ptr(), 8 if pos is None else pos.element_size(),
+            self.attention_factor, psb, pss, off, self._turns_on(dev))
+        with _lib.on_device(dev):
+            check(lib().vq_rotary(a, stream_ptr(dev)), fn)
 
     # -- calls ---------------------------------------------------------------------------
     def __call__(self, q: torch.Tensor, k: torch.Tensor | None = None, positions=None, *, inverse: bool = False):
@@ -216,18 +222,17 @@ class RotaryEmbedding:
 
     def _rotate(self, fn, q, k, positions, inverse):
         require_cuda(q, f"{fn}: q")
-        pairs, out = [], []
-        for x in (q, k):
-            if x is None:
-                out.append(None)
-                continue
-            if x.stride(3) != 1:
-                x = x.contiguous()
-            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            pairs.append((x, y))
-            out.append(y)
-        self._launch(fn, q.shape[0], q.shape[2], q.dtype, q.device, pairs, positions, inverse)
-        return tuple(out)
+        if q.stride(3) != 1:
+            q = q.contiguous()
+        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if k is None:
+            self._launch(fn, q, yq, None, 0, _NONE[:3], None, 0, _NONE[:3], positions, inverse)
+            return yq, None
+        if k.stride(3) != 1:
+            k = k.contiguous()
+        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        self._launch(fn, q, yq, k, yk.data_ptr(), yk.stride()[:3], None, 0, _NONE[:3], positions, inverse)
+        return yq, yk
 
     def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_res: torch.Tensor, v_res: torch.Tensor, tok_offset: int,
                positions=None) -> torch.Tensor:
@@ -240,24 +245,34 @@ class RotaryEmbedding:
         self._check_append(q, k, v)
         B, H, S, D = k.shape
         for name, t in (("k_res", k_res), ("v_res", v_res)):
-            if t.ndim != 4 or t.shape[0] != B or t.shape[1] != H or t.shape[3] != D or t.dtype is not k.dtype or t.device != k.device:
-                raise ValueError(f"{fn}: {name} must be [{B}, {H}, rows, {D}] {k.dtype} on {k.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-            if t.stride(3) != 1 or t.stride(2) < D or 0 in t.stride()[:2]:
-                raise ValueError(f"{fn}: the channels of {name} must be contiguous and its rows apart, got strides {t.stride()}")
-            if tok_offset < 0 or tok_offset + S > t.shape[2]:
-                raise ValueError(f"{fn}: rows [{tok_offset}, {tok_offset + S}) exceed {name} ({t.shape[2]} rows)")
+            shape, stride = t.shape, t.stride()
+            if len(shape) != 4 or shape[0] != B or shape[1] != H or shape[3] != D or t.dtype is not k.dtype or t.device != k.device:
+                raise ValueError(f"{fn}: {name} must be [{B}, {H}, rows, {D}] {k.dtype} on {k.device}, got {tuple(shape)} {t.dtype} on {t.device}")
+            if stride[3] != 1 or stride[2] < D or not stride[0] or not stride[1]:
+                raise ValueError(f"{fn}: the channels of {name} must be contiguous and its rows apart, got strides {stride}")
+            if tok_offset < 0 or tok_offset + S > shape[2]:
+                raise ValueError(f"{fn}: rows [{tok_offset}, {tok_offset + S}) exceed {name} ({shape[2]} rows)")
         require_cuda(q, f"{fn}: q")
-        q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
+        if q.stride(3) != 1:
+            q = q.contiguous()
+        if k.stride(3) != 1:
+            k = k.contiguous()
+        if v.stride(3) != 1:
+            v = v.contiguous()
         if k_res.data_ptr() == v_res.data_ptr():
             raise ValueError(f"{fn}: k_res and v_res must be different memory")
-        held = {k_res.untyped_storage().data_ptr(), v_res.untyped_storage().data_ptr()}
-        if any(t.untyped_storage().data_ptr() in held for t in (q, k, v)):
+        held = (k_res.untyped_storage().data_ptr(), v_res.untyped_storage().data_ptr())
+        if q.untyped_storage().data_ptr() in held or k.untyped_storage().data_ptr() in held or v.untyped_storage().data_ptr() in held:
             raise ValueError(f"{fn}: q, k and v must not share memory with k_res / v_res")
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         es = k.element_size()
-        rows = [(t.data_ptr() + tok_offset * t.stride(2) * es, t.stride()) for t in (k_res, v_res)]
-        self._launch(fn, B, S, q.dtype, q.device, ((q, out), (k, rows[0]), (v, rows[1])), positions, False)
+        ks, vs = k_res.stride(), v_res.stride()
+        self._launch(fn, q, out, k, k_res.data_ptr() + tok_offset * ks[2] * es, ks[:3], v, v_res.data_ptr() + tok_offset * vs[2] * es, vs[:3], positions, False)
         return out
+
+
+def _turn(rope, positions, inverse, q, k):
+    return rope._rotate("RotaryEmbedding", q, k, positions, inverse)
 
 
 class _Rotate(torch.autograd.Function):
@@ -272,19 +287,19 @@ class _Rotate(torch.autograd.Function):
             ctx.save_for_backward(positions)
         else:
             ctx.positions = positions
-        return rope._rotate("RotaryEmbedding", q, k, positions, inverse)
+        return _turn(rope, positions, inverse, q, k)
 
     @staticmethod
     def backward(ctx, gq, gk):
         positions = ctx.saved_tensors[0] if ctx.tensor_positions else ctx.positions
         need_q, need_k = ctx.needs_input_grad[3], ctx.needs_input_grad[4]
         gq, gk = gq if need_q else None, gk if need_k else None
-        if gq is not None and gk is not None:
-            gq, gk = _Rotate.apply(ctx.rope, positions, not ctx.inverse, gq, gk)
-        elif gq is not None:
-            gq = _Rotate.apply(ctx.rope, positions, not ctx.inverse, gq, None)[0]
+        # (through the function again only where a second derivative may be asked for)
+        turn = _Rotate.apply if torch.is_grad_enabled() else _turn
+        if gq is not None:
+            gq, gk = turn(ctx.rope, positions, not ctx.inverse, gq, gk)
         elif gk is not None:
-            gk = _Rotate.apply(ctx.rope, positions, not ctx.inverse, gk, None)[0]
+            gk = turn(ctx.rope, positions, not ctx.inverse, gk, None)[0]
         return None, None, None, gq, gk
 
 

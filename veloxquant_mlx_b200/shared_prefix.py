@@ -15,7 +15,7 @@ from typing import Any
 import torch
 
 from . import _lib
-from ._lib import KiviRowsArgs, SharedAttendArgs, check, lib, require_cuda, stream_ptr
+from ._lib import KIVI_ROWS_PACK, SHARED_ATTEND_HEAD, SHARED_ATTEND_TAIL, check, lib, require_cuda, stream_ptr
 
 _GROUP = 32
 
@@ -61,8 +61,8 @@ class KiviRows:
                 raise ValueError(f"{fn}: {name} must be contiguous")
             if t.device != first.device:
                 raise ValueError(f"{fn}: {name} is on {t.device}, {tensors[0][0]} on {first.device}")
-        a = KiviRowsArgs()
         cap = cap_res = 0
+        pointers, strides, res_stride = (0,) * 6, (0,) * 4, 0
         if k_codes is not None:
             rb = D * store_bits // 8
             if k_codes.dtype != torch.uint8 or v_codes.dtype != torch.uint8 or k_codes.shape[3] != rb or v_codes.shape[3] != rb:
@@ -75,15 +75,12 @@ class KiviRows:
             if v_scale.shape != v_zero.shape or v_scale.shape[3] != D // _GROUP:
                 raise ValueError(f"{fn}: v_scale / v_zero must be equal [{B}, {H}, tokens, {D // _GROUP}], got {tuple(v_scale.shape)} / {tuple(v_zero.shape)}")
             cap = min(cap, k_scale.shape[2] * _GROUP, v_scale.shape[2])
-            a.k_codes, a.v_codes, a.k_scale, a.k_zero = k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), k_zero.data_ptr()
-            a.v_scale, a.v_zero = v_scale.data_ptr(), v_zero.data_ptr()
+            pointers = tuple(t.data_ptr() for t in (k_codes, v_codes, k_scale, k_zero, v_scale, v_zero))
             if any(packed[n].data_ptr() % 16 for n in packed):
                 raise ValueError(f"{fn}: codes, scales and zeros must be 16-byte aligned")
             if k_codes.shape[2] != v_codes.shape[2]:
                 raise ValueError(f"{fn}: k_codes and v_codes must hold the same tokens, got {k_codes.shape[2]} and {v_codes.shape[2]}")
-            a.k_codes_stride_bh = a.v_codes_stride_bh = k_codes.shape[2] * rb
-            a.k_param_stride_bh = k_scale.shape[2] * D
-            a.v_param_stride_bh = v_scale.shape[2] * (D // _GROUP)
+            strides = (k_codes.shape[2] * rb, v_codes.shape[2] * rb, k_scale.shape[2] * D, v_scale.shape[2] * (D // _GROUP))
         self.dtype = None
         if k_res is not None:
             if k_res.dtype not in (torch.float16, torch.bfloat16) or v_res.dtype != k_res.dtype or v_res.shape != k_res.shape:
@@ -93,9 +90,9 @@ class KiviRows:
                 raise ValueError(f"{fn}: k_res / v_res must be 16-byte aligned")
             cap_res = k_res.shape[2]
             self.dtype = k_res.dtype
-            a.res_stride_bh = cap_res * D
+            res_stride = cap_res * D
         self.batch, self.heads, self.head_dim, self.store_bits, self.device = B, H, D, store_bits, first.device
-        self._cap, self._cap_res, self._args = cap, cap_res, a
+        self._cap, self._cap_res, self._pointers, self._strides = cap, cap_res, pointers, (*strides, res_stride)
         self._tensors = (k_codes, k_scale, k_zero, v_codes, v_scale, v_zero, k_res, v_res)  # (kept alive)
         self._k_res_ptr, self._v_res_ptr = (0, 0) if k_res is None else (k_res.data_ptr(), v_res.data_ptr())
         self.resize(cap // _GROUP * _GROUP if n_quant is None else n_quant, cap_res - res_offset if n_res is None else n_res, res_offset)
@@ -106,16 +103,16 @@ class KiviRows:
             raise ValueError(f"KiviRows: n_quant={n_quant} must be a multiple of 32 within the {self._cap} packed tokens held")
         if n_res < 0 or res_offset < 0 or res_offset + n_res > self._cap_res:
             raise ValueError(f"KiviRows: rows [{res_offset}, {res_offset + n_res}) exceed the exact rows ({self._cap_res})")
-        a, skip = self._args, res_offset * self.head_dim * 2
-        a.n_quant, a.n_res = n_quant, n_res
-        a.k_res, a.v_res = (self._k_res_ptr + skip, self._v_res_ptr + skip) if n_res else (None, None)
+        skip = res_offset * self.head_dim * 2
+        res = (self._k_res_ptr + skip, self._v_res_ptr + skip) if n_res else (0, 0)
+        self._args = KIVI_ROWS_PACK.pack(*self._pointers, *res, *self._strides, n_quant, n_res)
         self.n_quant, self.n_res = n_quant, n_res
 
     def __len__(self) -> int:
         return self.n_quant + self.n_res
 
 
-_EMPTY = KiviRowsArgs()
+_EMPTY = bytes(KIVI_ROWS_PACK.size)
 
 
 def kivi_shared_prefix_attend(q: torch.Tensor, prefix: KiviRows, own: KiviRows | None, scale: float, *, causal: bool = True,
@@ -146,17 +143,16 @@ def kivi_shared_prefix_attend(q: torch.Tensor, prefix: KiviRows, own: KiviRows |
         raise ValueError(f"{fn}: prefix and own must be KiviRows")
     if prefix.batch != 1:
         raise ValueError(f"{fn}: the prefix must have batch 1, got {prefix.batch}")
-    H_kv = prefix.heads
+    H_kv, bits = prefix.heads, prefix.store_bits
     dev = q.device
-    for name, st in (("prefix", prefix), ("own", own)):
-        if st is None:
-            continue
-        if st.head_dim != D or st.heads != H_kv or st.store_bits != prefix.store_bits:
-            raise ValueError(f"{fn}: {name} has {st.heads} heads of {st.head_dim} at {st.store_bits} bits; {H_kv} of {D} at {prefix.store_bits} expected")
+    for st in (prefix,) if own is None else (prefix, own):
+        if st.head_dim != D or st.heads != H_kv or st.store_bits != bits:
+            raise ValueError(f"{fn}: {'prefix' if st is prefix else 'own'} has {st.heads} heads of {st.head_dim} at {st.store_bits} bits; {H_kv} of {D} at "
+                             f"{bits} expected")
         if st.device != dev:
-            raise ValueError(f"{fn}: {name} is on {st.device}, q on {dev}")
+            raise ValueError(f"{fn}: {'prefix' if st is prefix else 'own'} is on {st.device}, q on {dev}")
         if st.n_res and st.dtype is not dt:
-            raise ValueError(f"{fn}: the exact rows of {name} are {st.dtype}, q is {dt}")
+            raise ValueError(f"{fn}: the exact rows of {'prefix' if st is prefix else 'own'} are {st.dtype}, q is {dt}")
     if own is not None and own.batch != B:
         raise ValueError(f"{fn}: own has batch {own.batch}, q {B}")
     if H % H_kv:
@@ -180,16 +176,15 @@ def kivi_shared_prefix_attend(q: torch.Tensor, prefix: KiviRows, own: KiviRows |
     if out.data_ptr() % 16:
         raise ValueError(f"{fn}: out must be 16-byte aligned")
     lse = torch.empty((B, H, S_q), dtype=torch.float32, device=dev) if return_lse else None
-    a = SharedAttendArgs(q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), None if own_start is None else own_start.data_ptr(),
-                         0 if dt is torch.float16 else 1, B, H, H_kv, S_q, D, prefix.store_bits, _GROUP, scale, _lib.VQ_ATTEND_CAUSAL if causal else 0,
-                         prefix._args, _EMPTY if own is None else own._args, None, 0, variant, n_splits)
+    head = SHARED_ATTEND_HEAD.pack(q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if own_start is None else own_start.data_ptr(),
+                                   0 if dt is torch.float16 else 1, B, H, H_kv, S_q, D, bits, _GROUP, scale, _lib.VQ_ATTEND_CAUSAL if causal else 0)
+    head += prefix._args + (_EMPTY if own is None else own._args)
     native = lib()
     with _lib.on_device(dev):
-        need = native.vq_kivi_shared_attend_workspace_bytes(a)
+        need = native.vq_kivi_shared_attend_workspace_bytes(head + SHARED_ATTEND_TAIL.pack(0, 0, variant, n_splits))
         # (from torch's allocator at every call: calls on other streams and captured graphs have their own)
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        check(native.vq_kivi_shared_attend(a, stream_ptr(dev)), fn)
+        check(native.vq_kivi_shared_attend(head + SHARED_ATTEND_TAIL.pack(ws.data_ptr(), need, variant, n_splits), stream_ptr(dev)), fn)
     return out if lse is None else (out, lse)
 
 
