@@ -24,6 +24,11 @@ _NONE = (0, 0, 0, 0)
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
+def _empty(x: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor like ``x`` (empty_like costs a third of torch.empty, but keeps strides)."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None) -> tuple[torch.Tensor, float]:
     """Angle per position of each of the ``rotary_dim / 2`` pairs (float64, on the host) and the
     factor on sine and cosine.
@@ -224,13 +229,13 @@ class RotaryEmbedding:
         require_cuda(q, f"{fn}: q")
         if q.stride(3) != 1:
             q = q.contiguous()
-        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        yq = _empty(q)
         if k is None:
             self._launch(fn, q, yq, None, 0, _NONE[:3], None, 0, _NONE[:3], positions, inverse)
             return yq, None
         if k.stride(3) != 1:
             k = k.contiguous()
-        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        yk = _empty(k)
         self._launch(fn, q, yq, k, yk.data_ptr(), yk.stride()[:3], None, 0, _NONE[:3], positions, inverse)
         return yq, yk
 
@@ -264,7 +269,7 @@ class RotaryEmbedding:
         held = (k_res.untyped_storage().data_ptr(), v_res.untyped_storage().data_ptr())
         if q.untyped_storage().data_ptr() in held or k.untyped_storage().data_ptr() in held or v.untyped_storage().data_ptr() in held:
             raise ValueError(f"{fn}: q, k and v must not share memory with k_res / v_res")
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = _empty(q)
         es = k.element_size()
         ks, vs = k_res.stride(), v_res.stride()
         self._launch(fn, q, out, k, k_res.data_ptr() + tok_offset * ks[2] * es, ks[:3], v, v_res.data_ptr() + tok_offset * vs[2] * es, vs[:3], positions, False)

@@ -165,7 +165,7 @@ def kivi_shared_prefix_attend(q: torch.Tensor, prefix: KiviRows, own: KiviRows |
     if q.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{fn}: not differentiable (q requires grad; call it under torch.no_grad())")
     if out is None:
-        out = torch.empty(q.shape, dtype=dt, device=dev)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=dev)
     elif out.shape != q.shape or out.dtype is not dt or out.device != dev or not out.is_contiguous():
         raise ValueError(f"{fn}: out must be a contiguous {tuple(q.shape)} {dt} tensor on {dev}")
     require_cuda(q, f"{fn}: q")
@@ -183,7 +183,7 @@ def kivi_shared_prefix_attend(q: torch.Tensor, prefix: KiviRows, own: KiviRows |
     with _lib.on_device(dev):
         need = native.vq_kivi_shared_attend_workspace_bytes(head + SHARED_ATTEND_TAIL.pack(0, 0, variant, n_splits))
         # (from torch's allocator at every call: calls on other streams and captured graphs have their own)
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        ws = q.new_empty(need // 2 + 8)
         check(native.vq_kivi_shared_attend(head + SHARED_ATTEND_TAIL.pack(ws.data_ptr(), need, variant, n_splits), stream_ptr(dev)), fn)
     return out if lse is None else (out, lse)
 
