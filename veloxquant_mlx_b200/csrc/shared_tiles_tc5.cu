@@ -26,6 +26,7 @@
 // Every wait is bounded; a role that gives up raises a flag (reported by vq_kivi_attend_status), leaves its
 // loop, and the CTA still waits (bounded) for its MMAs and frees its tensor memory.
 #include <algorithm>
+#include <type_traits>
 
 #include "shared_attend.h"
 
@@ -209,11 +210,40 @@ __device__ __forceinline__ uint4 decode8(const uint32_t (&w)[SB == 8 ? 2 : 1], c
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
+// The same in half precision, for bfloat16 data and codes of 2 or 4 bits: a code beside the exponent of 1024
+// is the half 1024 + code * 2^bit, one half FMA makes it the code, exactly, and another one the value. Scale and
+// zero are rounded to halves, so a value is off by up to three roundings of 2^-11 instead of one (together
+// less than a quarter of bfloat16's own 2^-8 in the mean), for 13 instructions instead of 20. float16 data
+// keeps the float32 form. Word i of the result holds channels i and i + 4: see in_order.
+template <int SB>
+__device__ __forceinline__ uint4 decode8_half(uint32_t w, const uint32_t (&sc)[4], const uint32_t (&ze)[4]) {
+    uint32_t r[4];
+    if constexpr (SB == 2) w = __byte_perm(w, 0u, 0x4140);  // codes 0-3 into the low half, 4-7 into the high one
+    const uint32_t w8 = w >> 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int bit = SB == 2 ? 2 * i : 4 * (i & 1);
+        const uint32_t mask = (SB == 2 ? 0x00030003u : 0x000f000fu) << bit;
+        const uint32_t x = ((SB == 4 && i >= 2 ? w8 : w) & mask) | 0x64006400u;
+        // code = x * 2^-bit - 1024 * 2^-bit
+        const uint32_t down = 0x3c003c00u - (uint32_t)bit * 0x04000400u, off = 0xe400e400u - (uint32_t)bit * 0x04000400u;
+        r[i] = hfma2(hfma2(x, down, off), sc[i], ze[i]);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+// 8 halves in the order in which a tile holds a chunk's channels: as they come, or 0 4 1 5 2 6 3 7
+template <bool SPREAD>
+__device__ __forceinline__ uint4 in_order(uint4 v) {
+    if constexpr (!SPREAD) return v;
+    return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+}
+
 template <int D, int SB, typename T>
 __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __grid_constant__ TileParams p) {
     using L = Layout<D>;
     constexpr int CHUNKS = D / 8;      // 8-channel chunks of a row
     constexpr int RB = D * SB / 8;     // bytes of a packed row
+    constexpr bool HALF = std::is_same<T, __nv_bfloat16>::value && SB != 8;  // decode8_half; channels of a chunk spread
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -271,14 +301,24 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
     if (warp < 8) {
         // ---- softmax: thread = row -----------------------------------------------------------------
         // first the query tiles, as halves; rows behind the last are zero
-        for (int i = tid; i < (two ? 2 : 1) * kTile * CHUNKS; i += 256) {
-            const int r = i / CHUNKS, c = i % CHUNKS;
-            uint4 v = zero4();
-            if (row0 + r < n_rows) {
-                v = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(p.q) + out_row(row0 + r) * D) + c);
-                v = make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w));
+        // (eight loads in flight a thread: one by one they would take longer than several token tiles)
+        constexpr int STEP = 256 / CHUNKS;  // rows that the 256 threads cover at once
+        const int qc = tid % CHUNKS;
+#pragma unroll 1
+        for (int r0 = tid / CHUNKS; r0 < (two ? 2 : 1) * kTile; r0 += 8 * STEP) {
+            uint4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = r0 + i * STEP;
+                v[i] = zero4();
+                if (row0 + r < n_rows) v[i] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(p.q) + out_row(row0 + r) * D) + qc);
             }
-            *reinterpret_cast<uint4 *>(smem + L::Q + (r / kTile) * L::TILE + L::at(r % kTile, c)) = v;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = r0 + i * STEP;
+                *reinterpret_cast<uint4 *>(smem + L::Q + (r / kTile) * L::TILE + L::at(r % kTile, qc)) =
+                    in_order<HALF>(make_uint4(as_f16x2<T>(v[i].x), as_f16x2<T>(v[i].y), as_f16x2<T>(v[i].z), as_f16x2<T>(v[i].w)));
+            }
         }
         ready();
         const int s = warp >> 2;
@@ -368,8 +408,12 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
             tmem_ld32(to + c, v);
             tmem_ld_wait(v);
 #pragma unroll
-            for (int k = 0; k < 32; k += 4)
-                *reinterpret_cast<float4 *>(mine + 4 * (c + k)) = n_mine > 0 ? make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < 32; k += 4) {
+                const int k8 = k & ~7, odd = k >> 2 & 1;  // channel k + i of the output is column k8 + 2 i + odd of a spread chunk
+                *reinterpret_cast<float4 *>(mine + 4 * (c + k)) = n_mine == 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                                  : HALF ? make_float4(v[k8 + odd], v[k8 + 2 + odd], v[k8 + 4 + odd], v[k8 + 6 + odd])
+                                                                         : make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+            }
         }
         fence_async_smem();
         if (live) {
@@ -425,17 +469,26 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
             const int t = t_lo + i, stage = i & 1;
             if (t < tiles_packed) {
                 const bool some = here(t), more = here(t + 1);
-                const float2 sc[4] = {{ns[0].x, ns[0].y}, {ns[0].z, ns[0].w}, {ns[1].x, ns[1].y}, {ns[1].z, ns[1].w}};
-                const float2 zz[4] = {{nz[0].x, nz[0].y}, {nz[0].z, nz[0].w}, {nz[1].x, nz[1].y}, {nz[1].z, nz[1].w}};
-                float2 ze[4];
+                float2 sc[4], ze[4];
+                uint32_t sh[4], zh[4];
+                if constexpr (HALF) {
+                    const float s8[8] = {ns[0].x, ns[0].y, ns[0].z, ns[0].w, ns[1].x, ns[1].y, ns[1].z, ns[1].w};
+                    const float z8[8] = {nz[0].x, nz[0].y, nz[0].z, nz[0].w, nz[1].x, nz[1].y, nz[1].z, nz[1].w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) ze[k] = fma2(make_float2(-Codes<SB>::kBase, -Codes<SB>::kBase), sc[k], zz[k]);
+                    for (int k = 0; k < 4; ++k) { sh[k] = pack_f16(s8[k], s8[k + 4]); zh[k] = pack_f16(z8[k], z8[k + 4]); }
+                } else {
+                    sc[0] = {ns[0].x, ns[0].y}; sc[1] = {ns[0].z, ns[0].w}; sc[2] = {ns[1].x, ns[1].y}; sc[3] = {ns[1].z, ns[1].w};
+                    const float2 zz[4] = {{nz[0].x, nz[0].y}, {nz[0].z, nz[0].w}, {nz[1].x, nz[1].y}, {nz[1].z, nz[1].w}};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) ze[k] = fma2(make_float2(-Codes<SB>::kBase, -Codes<SB>::kBase), sc[k], zz[k]);
+                }
                 if (more) fetch_params(t + 1);
                 if (i >= 2 && !wait(kKEmpty + stage, ((i >> 1) - 1) & 1)) break;
                 if (some) {
 #pragma unroll
                     for (int k = 0; k < N; ++k) {
-                        *reinterpret_cast<uint4 *>(place(stage, k)) = decode8<SB>(cur[k], sc, ze);
+                        if constexpr (HALF) *reinterpret_cast<uint4 *>(place(stage, k)) = decode8_half<SB>(cur[k][0], sh, zh);
+                        else *reinterpret_cast<uint4 *>(place(stage, k)) = decode8<SB>(cur[k], sc, ze);
                         if (more) fetch_codes(t + 1, k);
                     }
                 } else {
@@ -451,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
                     uint4 v = zero4();
                     if (row < st.n_res) {
                         v = __ldg(reinterpret_cast<const uint4 *>(exact + (int64_t)row * D) + chunk);
-                        v = make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w));
+                        v = in_order<HALF>(make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w)));
                     }
                     *reinterpret_cast<uint4 *>(place(stage, k)) = v;
                 }
@@ -506,13 +559,18 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
                     const bool some = here(t, k) && t * kTile + k * TPI + tok >= first_slot;
                     const float sk = sc[k], zk = fmaf(-Codes<SB>::kBase, sc[k], ze[k]);
                     const float2 s8[4] = {{sk, sk}, {sk, sk}, {sk, sk}, {sk, sk}}, z8[4] = {{zk, zk}, {zk, zk}, {zk, zk}, {zk, zk}};
+                    const uint32_t s2 = pack_f16(sc[k], sc[k]), z2 = pack_f16(ze[k], ze[k]);
+                    const uint32_t sh[4] = {s2, s2, s2, s2}, zh[4] = {z2, z2, z2, z2};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t wd[SB == 8 ? 2 : 1];
                         if constexpr (SB == 8) { wd[0] = cur[k][2 * j]; wd[1] = cur[k][2 * j + 1]; }
                         else if constexpr (SB == 4) wd[0] = cur[k][j];
                         else wd[0] = cur[k][j / 2] >> (16 * (j & 1));
-                        *reinterpret_cast<uint4 *>(place(stage, k, j)) = some ? decode8<SB>(wd, s8, z8) : zero4();
+                        uint4 v;
+                        if constexpr (HALF) v = decode8_half<SB>(wd[0], sh, zh);
+                        else v = decode8<SB>(wd, s8, z8);
+                        *reinterpret_cast<uint4 *>(place(stage, k, j)) = some ? v : zero4();
                     }
                     if (here(t + 1, k)) fetch(t + 1, k);
                 }
@@ -527,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
                         uint4 v = zero4();
                         if (r0 + row < st.n_res && st.n_quant + r0 + row >= first_slot) {
                             v = __ldg(reinterpret_cast<const uint4 *>(exact + (int64_t)(r0 + row) * D) + 4 * grp + j);
-                            v = make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w));
+                            v = in_order<HALF>(make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w)));
                         }
                         *reinterpret_cast<uint4 *>(place(stage, k, j)) = v;
                     }
