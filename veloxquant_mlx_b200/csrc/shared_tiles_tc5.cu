@@ -177,6 +177,17 @@ struct TileParams {
     Part prefix, own;
 };
 
+// The block is launched with 96 registers a thread; where decoding needs fewer, the two softmax warpgroups
+// take over what the two decoding ones can spare (their sum is what the four were launched with).
+template <bool SPARE>
+__device__ __forceinline__ void more_registers() {
+    if constexpr (SPARE) asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
+}
+template <bool SPARE>
+__device__ __forceinline__ void fewer_registers() {
+    if constexpr (SPARE) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+}
+
 template <int D>
 struct Layout {
     static constexpr int HALVES = D / 64;                     // 64-channel (128-byte) halves of a tile
@@ -192,7 +203,7 @@ struct Layout {
     __device__ static __forceinline__ uint32_t at(int r, int c) { return (uint32_t)((c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 };
 
-enum { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPReady = 10, kODone = 12, kDrain = 14, kBars = 15 };
+enum { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPReady = 10, kPVHalf = 14, kODone = 16, kDrain = 18, kBars = 19 };
 
 __device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
 
@@ -300,27 +311,34 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
     // scores (and the weights over them) of stream s: columns 128 s of tensor memory; its output: 256 + 128 s
     if (warp < 8) {
         // ---- softmax: thread = row -----------------------------------------------------------------
-        // first the query tiles, as halves; rows behind the last are zero
-        // (eight loads in flight a thread: one by one they would take longer than several token tiles)
+        // First the query tiles: copied as they are (all in flight at once), then made halves in place; rows
+        // behind the last are zero. (Small loops: code that runs once is fetched from L2 line by line.)
         constexpr int STEP = 256 / CHUNKS;  // rows that the 256 threads cover at once
-        const int qc = tid % CHUNKS;
+        const int qc = tid % CHUNKS, q_rows = (two ? 2 : 1) * kTile;
+        auto q_at = [&](int r) { return smem + L::Q + (r / kTile) * L::TILE + L::at(r % kTile, qc); };
+        int b = (row0 + tid / CHUNKS) / per_req, rem = row0 + tid / CHUNKS - b * per_req;  // (own: b = 0)
+        const int step_b = STEP / per_req, step_rem = STEP - step_b * per_req;
 #pragma unroll 1
-        for (int r0 = tid / CHUNKS; r0 < (two ? 2 : 1) * kTile; r0 += 8 * STEP) {
-            uint4 v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = r0 + i * STEP;
-                v[i] = zero4();
-                if (row0 + r < n_rows) v[i] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(p.q) + out_row(row0 + r) * D) + qc);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = r0 + i * STEP;
-                *reinterpret_cast<uint4 *>(smem + L::Q + (r / kTile) * L::TILE + L::at(r % kTile, qc)) =
-                    in_order<HALF>(make_uint4(as_f16x2<T>(v[i].x), as_f16x2<T>(v[i].y), as_f16x2<T>(v[i].z), as_f16x2<T>(v[i].w)));
+        for (int r = tid / CHUNKS; r < q_rows; r += STEP) {
+            const bool in = row0 + r < n_rows;
+            const int64_t row = ((int64_t)(b_own + b) * p.H_q + (int64_t)hk * p.G) * p.S_q + rem;
+            const T *src = reinterpret_cast<const T *>(p.q) + (in ? row : 0) * D + 8 * qc;
+            b += step_b;
+            rem += step_rem;
+            if (rem >= per_req) { rem -= per_req; ++b; }
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(q_at(r))), "l"(src), "r"(in ? 16 : 0) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if constexpr (HALF || std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll 4
+            for (int r = tid / CHUNKS; r < q_rows; r += STEP) {
+                uint4 *at = reinterpret_cast<uint4 *>(q_at(r));
+                const uint4 v = *at;
+                *at = in_order<HALF>(make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w)));
             }
         }
         ready();
+        more_registers<HALF>();
         const int s = warp >> 2;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + 128 * s + lane_base, to = ts + 256;
@@ -328,13 +346,15 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
         const int r = row0 + (two ? s * kTile : 0) + (warp & 3) * 32 + lane;
         // slots [first_slot, lim) are seen by this row
         const int lim = is_prefix || !p.causal ? n_slots : n_slots - p.S_q + r % p.S_q + 1;
+        // (tiles within [first_slot, the warp's smallest lim) need no mask)
+        const int all_see = __reduce_min_sync(0xffffffffu, lim);
         float m = -INFINITY, l = 0.f;  // reference maximum (times scale, base 2) and the weights' sum
         for (int i = 0; i < n_mine; ++i) {
             const int t = t_lo + (two ? i : 2 * i + s);
             const int slot0 = t < tiles_packed ? t * kTile : st.n_quant + (t - tiles_packed) * kTile;
             // columns [lo, hi) of the tile
             const int lo = first_slot - slot0, hi = min(lim, t < tiles_packed ? st.n_quant : n_slots) - slot0;
-            const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < kTile);
+            const bool masked = slot0 < first_slot || slot0 + kTile > (t < tiles_packed ? min(all_see, st.n_quant) : all_see);
             if (!wait(kSFull + s, i & 1)) break;
             fence_after();
             float2 sum[2] = {};
@@ -357,13 +377,16 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
                     l *= f;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) { sum[k].x *= f; sum[k].y *= f; }
-                    if (i > 0) {
+                    // (weights of the first half may have been taken by now: O holds them once that P V is done)
+                    if (c >= kTile / 2) wait(kPVHalf + s, i & 1);
+                    if (i > 0 || c >= kTile / 2) {
+                        fence_after();
 #pragma unroll 1
                         for (int k = 0; k < D; k += 8) scale_o(to + k, f);
                     }
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 #pragma unroll 1
-                    for (int k = 0; k < c / 2; k += 8) scale_p(ts + k, f);
+                    for (int k = c & (kTile / 2); k < c; k += 16) scale_p(ts + k / 2, f);
                 }
                 const float base = m == -INFINITY ? 0.f : -m;
                 uint32_t r[16];
@@ -387,12 +410,12 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
                 tmem_ld_wait(w);
                 if (c + 64 < kTile) tmem_ld32(ts + c + 64, v);
                 chunk(c + 32, w);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(kPReady + 2 * s + (c >> 6)));  // half of the weights
             }
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(kPReady + s));
         }
         // O goes out through shared memory: a row a lane there, whole rows at a time to global memory. The
         // tiles it overwrites are done with when both streams are.
@@ -403,17 +426,17 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
         const int64_t rec = live ? out_row(r) * p.parts.n_splits + part.record0 + (two ? split : 2 * split + s) : 0;
         uint8_t *mine = smem + (warp * 32 + lane) * L::OUT_ROW;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-            float v[32];
-            tmem_ld32(to + c, v);
-            tmem_ld_wait(v);
+        for (int c = 0; c < D; c += 8) {
+            uint32_t v[8];
+            tmem_ld8(to + c, v);
+            if (n_mine == 0) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-                const int k8 = k & ~7, odd = k >> 2 & 1;  // channel k + i of the output is column k8 + 2 i + odd of a spread chunk
-                *reinterpret_cast<float4 *>(mine + 4 * (c + k)) = n_mine == 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                                  : HALF ? make_float4(v[k8 + odd], v[k8 + 2 + odd], v[k8 + 4 + odd], v[k8 + 6 + odd])
-                                                                         : make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                for (int k = 0; k < 8; ++k) v[k] = 0u;
             }
+            // (channels i and i + 4 of a spread chunk are columns 2 i and 2 i + 1)
+            uint4 *at = reinterpret_cast<uint4 *>(mine + 4 * c);
+            at[0] = HALF ? make_uint4(v[0], v[2], v[4], v[6]) : make_uint4(v[0], v[1], v[2], v[3]);
+            at[1] = HALF ? make_uint4(v[1], v[3], v[5], v[7]) : make_uint4(v[4], v[5], v[6], v[7]);
         }
         fence_async_smem();
         if (live) {
@@ -423,6 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     } else if (warp < 12) {
+        fewer_registers<HALF>();
         // ---- keys: warp w decodes the w-th 32-token group of a tile -----------------------------------
         // lane = (token parity, chunk of 8 channels): the group's scales and zeros of 8 channels stay in registers
         constexpr int TPL = 32 / CHUNKS;          // tokens a warp covers at once: 2 (D = 128) or 4
@@ -459,12 +483,12 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
         auto place = [&](int stage, int k) { return smem + L::K + stage * L::TILE + ((at0 ^ ((TPL * k & 7) << 4)) + TPL * k * 128); };
         if (warp == 8 && elect_one()) {
             for (int i = 0; i < kBars; ++i) {
-                const bool by_warps = i < kKEmpty || (i >= kVFull && i < kVEmpty) || (i >= kPReady && i < kODone);
+                const bool by_warps = i < kKEmpty || (i >= kVFull && i < kVEmpty) || (i >= kPReady && i < kPVHalf);
                 mbar_init(bar(i), by_warps ? 4 : 1);
             }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        ready();
+        if (n_tiles == 0) ready();
         for (int i = 0; i < n_tiles; ++i) {
             const int t = t_lo + i, stage = i & 1;
             if (t < tiles_packed) {
@@ -509,17 +533,21 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
                     *reinterpret_cast<uint4 *>(place(stage, k)) = v;
                 }
             }
+            if (i == 0) ready();  // (the first tile needs nothing of the others)
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kKFull + stage));
         }
     } else if (warp < 16) {
+        fewer_registers<HALF>();
         // ---- values: a thread decodes one 32-channel group (one scale, one zero) of a token ------------
         constexpr int GV = D / kGroup;            // value groups of a token = threads of a token
         constexpr int TPI = 128 / GV;             // tokens the four warps cover at once
         constexpr int N = kTile / TPI;            // tokens a thread decodes
         constexpr int W = SB;                     // words of 32 codes
-        const int vt = tid - 12 * 32, grp = vt % GV, tok = vt / GV;
+        // (D = 128: the eight lanes of a quarter-warp store to eight different 16-byte columns)
+        const int grp = D == 128 ? (lane & 1) | (lane >> 2 & 2) : lane & 1;
+        const int tok = (warp - 12) * (32 / GV) + (D == 128 ? (lane >> 1 & 3) | (lane >> 2 & 4) : lane >> 1);
         const uint8_t *codes = st.v_codes + unit * st.v_codes_stride_bh;
         const float *vs = st.v_scale + unit * st.v_param_stride_bh, *vz = st.v_zero + unit * st.v_param_stride_bh;
         const T *exact = reinterpret_cast<const T *>(st.v_res) + unit * st.res_stride_bh;
@@ -548,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
         // (row k TPI + tok, chunk 4 grp + j: TPI is a multiple of 8, so only j moves the place)
         const uint32_t at0 = L::at(tok, 4 * grp);
         auto place = [&](int stage, int k, int j) { return smem + L::V + stage * L::TILE + ((at0 ^ (j << 4)) + k * TPI * 128); };
-        ready();
+        if (n_tiles == 0) ready();
         for (int i = 0; i < n_tiles; ++i) {
             const int t = t_lo + i, stage = i & 1;
             if (t < tiles_packed) {
@@ -591,6 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
                     }
                 }
             }
+            if (i == 0) ready();
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kVFull + stage));
@@ -625,13 +654,21 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
         auto pv = [&](int j) {
             const int s = j & 1, t = two ? j >> 1 : j, stage = t & 1;
             if ((!two || s == 0) && !wait(kVFull + stage, (t >> 1) & 1)) return;
-            if (!wait(kPReady + s, (j >> 1) & 1)) return;
-            fence_after();
             const uint64_t b = dv + stage * (L::TILE >> 4);
             const uint32_t d = tmem + 256 + 128 * s, a = tmem + 128 * s;
-            if (elected) {
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+                if (!wait(kPReady + 2 * s + half, (j >> 1) & 1)) return;
+                fence_after();
+                if (elected) {
 #pragma unroll
-                for (int k = 0; k < kTile / 16; ++k) mma_ts(d, a + 8 * k, b + k * (2048 >> 4), make_idesc(D, true), j >= 2 || k > 0);
+                    for (int k = 0; k < kTile / 32; ++k)
+                        mma_ts(d, a + 32 * half + 8 * k, b + half * (kTile / 2 * 128 >> 4) + k * (2048 >> 4), make_idesc(D, true), j >= 2 || half > 0 || k > 0);
+                    if (half == 0) mma_commit(bar(kPVHalf + s));
+                }
+                __syncwarp();
+            }
+            if (elected) {
                 if (!two || s == 1) mma_commit(bar(kVEmpty + stage));
                 if (j + 2 >= n_steps) mma_commit(bar(kODone + s));
             }
