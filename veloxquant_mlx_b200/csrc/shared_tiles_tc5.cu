@@ -424,27 +424,31 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
         fence_after();
         const bool live = r < n_rows;
         const int64_t rec = live ? out_row(r) * p.parts.n_splits + part.record0 + (two ? split : 2 * split + s) : 0;
-        uint8_t *mine = smem + (warp * 32 + lane) * L::OUT_ROW;
+        uint8_t *rows = smem + warp * 32 * L::OUT_ROW, *mine = rows + lane * L::OUT_ROW;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 8) {
-            uint32_t v[8];
-            tmem_ld8(to + c, v);
-            if (n_mine == 0) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = 0u;
-            }
+        for (int c = 0; c < D; c += 32) {
+            float v[32];
+            tmem_ld32(to + c, v);
+            tmem_ld_wait(v);
             // (channels i and i + 4 of a spread chunk are columns 2 i and 2 i + 1)
-            uint4 *at = reinterpret_cast<uint4 *>(mine + 4 * c);
-            at[0] = HALF ? make_uint4(v[0], v[2], v[4], v[6]) : make_uint4(v[0], v[1], v[2], v[3]);
-            at[1] = HALF ? make_uint4(v[1], v[3], v[5], v[7]) : make_uint4(v[4], v[5], v[6], v[7]);
+            float4 *at = reinterpret_cast<float4 *>(mine + 4 * c);
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+                at[k / 4] = HALF ? make_float4(v[k], v[k + 2], v[k + 4], v[k + 6]) : make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                at[k / 4 + 1] = HALF ? make_float4(v[k + 1], v[k + 3], v[k + 5], v[k + 7]) : make_float4(v[k + 4], v[k + 5], v[k + 6], v[k + 7]);
+            }
         }
-        fence_async_smem();
-        if (live) {
-            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.parts.o + rec * D), "r"(smem_u32(mine)), "n"(4 * D) : "memory");
-            *reinterpret_cast<float2 *>(p.parts.ml + rec * 2) = make_float2(m, l);
+        if (live) *reinterpret_cast<float2 *>(p.parts.ml + rec * 2) = make_float2(m, l);
+        __syncwarp();
+        constexpr int LPR = D / 4;  // lanes that write a row
+#pragma unroll 4
+        for (int i = 0; i < 32; i += 32 / LPR) {
+            const int from = i + lane / LPR;
+            const float4 v = *reinterpret_cast<const float4 *>(rows + from * L::OUT_ROW + 16 * (lane % LPR));
+            const int64_t to_rec = __shfl_sync(0xffffffffu, rec, from);
+            if (row0 + (two ? s * kTile : 0) + (warp & 3) * 32 + from < n_rows)
+                *reinterpret_cast<float4 *>(p.parts.o + to_rec * D + 4 * (lane % LPR)) = n_mine > 0 ? v : make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     } else if (warp < 12) {
         fewer_registers<HALF>();
         // ---- keys: warp w decodes the w-th 32-token group of a tile -----------------------------------
