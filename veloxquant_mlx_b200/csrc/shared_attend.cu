@@ -101,6 +101,8 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
     constexpr int GV = S::GV, RB = S::RB;
     constexpr int ROWS = 8 * NT;
     constexpr float BASE = Codes<SB>::kBase;
+    // codes through half precision (half_codes); a lane's channels 8 j + i of K then pair with 8 j + i + 4
+    constexpr bool HALF = std::is_same<T, __nv_bfloat16>::value && SB != 8;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float sh_m[kWarps][ROWS], sh_l[kWarps][ROWS];
     let_next_start();
@@ -192,8 +194,8 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
 #pragma unroll
             for (int i = 0; i < CH / 8; ++i) {
                 const uint4 v = __ldg(src + i);
-                qb[nt][4 * i] = as_f16x2<T>(v.x); qb[nt][4 * i + 1] = as_f16x2<T>(v.y);
-                qb[nt][4 * i + 2] = as_f16x2<T>(v.z); qb[nt][4 * i + 3] = as_f16x2<T>(v.w);
+                const uint4 w = in_order<HALF>(make_uint4(as_f16x2<T>(v.x), as_f16x2<T>(v.y), as_f16x2<T>(v.z), as_f16x2<T>(v.w)));
+                qb[nt][4 * i] = w.x; qb[nt][4 * i + 1] = w.y; qb[nt][4 * i + 2] = w.z; qb[nt][4 * i + 3] = w.w;
             }
         }
 #pragma unroll
@@ -266,26 +268,54 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
             uint32_t w[4][KW];
 #pragma unroll
             for (int j = 0; j < 4; ++j) lds(w[j], buf + S::KC + (8 * j + tau) * RB + c4 * (CH * SB / 8));
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const int at = 16 * S::param_chunk(c4 * (CH / 4) + k);
-                const float4 sc = *reinterpret_cast<const float4 *>(buf + S::KS + at), zz = *reinterpret_cast<const float4 *>(buf + S::KZ + at);
-                const float2 s0 = make_float2(sc.x, sc.y), s1 = make_float2(sc.z, sc.w), nb = make_float2(-BASE, -BASE);
-                const float2 z0 = fma2(nb, s0, make_float2(zz.x, zz.y)), z1 = fma2(nb, s1, make_float2(zz.z, zz.w));
-                uint32_t a[4][2];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t word = w[j][4 * k / Codes<SB>::kPerWord];
-                    const int i0 = 4 * k % Codes<SB>::kPerWord;
-                    const float2 x = fma2(make_float2(Codes<SB>::get(word, i0), Codes<SB>::get(word, i0 + 1)), s0, z0);
-                    const float2 y = fma2(make_float2(Codes<SB>::get(word, i0 + 2), Codes<SB>::get(word, i0 + 3)), s1, z1);
-                    a[j][0] = pack_f16(x.x, x.y);
-                    a[j][1] = pack_f16(y.x, y.y);
-                }
+            auto qk = [&](int k, const uint32_t (&a)[4][2]) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     mma16816(s[nt][0], a[0][0], a[1][0], a[0][1], a[1][1], qb[nt][2 * k], qb[nt][2 * k + 1]);
                     mma16816(s[nt][1], a[2][0], a[3][0], a[2][1], a[3][1], qb[nt][2 * k], qb[nt][2 * k + 1]);
+                }
+            };
+            if constexpr (HALF) {
+#pragma unroll
+                for (int k = 0; k < KS; k += 2) {  // eight channels: pairs (0, 4) (1, 5) to one MMA, (2, 6) (3, 7) to the next
+                    float4 sc[2], ze[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int at = 16 * S::param_chunk(c4 * (CH / 4) + k + i);
+                        sc[i] = *reinterpret_cast<const float4 *>(buf + S::KS + at);
+                        ze[i] = *reinterpret_cast<const float4 *>(buf + S::KZ + at);
+                    }
+                    const uint32_t sh[4] = {pack_f16(sc[0].x, sc[1].x), pack_f16(sc[0].y, sc[1].y), pack_f16(sc[0].z, sc[1].z), pack_f16(sc[0].w, sc[1].w)};
+                    const uint32_t zh[4] = {pack_f16(ze[0].x, ze[1].x), pack_f16(ze[0].y, ze[1].y), pack_f16(ze[0].z, ze[1].z), pack_f16(ze[0].w, ze[1].w)};
+                    uint32_t a[2][4][2];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t word = SB == 4 ? w[j][k / 2] : __byte_perm(w[j][k / 4], 0u, k / 2 % 2 ? 0x4342 : 0x4140);
+                        const uint32_t w8 = word >> 8;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) a[i >> 1][j][i & 1] = hfma2(half_codes<SB>(word, w8, i), sh[i], zh[i]);
+                    }
+                    qk(k, a[0]);
+                    qk(k + 1, a[1]);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    const int at = 16 * S::param_chunk(c4 * (CH / 4) + k);
+                    const float4 sc = *reinterpret_cast<const float4 *>(buf + S::KS + at), zz = *reinterpret_cast<const float4 *>(buf + S::KZ + at);
+                    const float2 s0 = make_float2(sc.x, sc.y), s1 = make_float2(sc.z, sc.w), nb = make_float2(-BASE, -BASE);
+                    const float2 z0 = fma2(nb, s0, make_float2(zz.x, zz.y)), z1 = fma2(nb, s1, make_float2(zz.z, zz.w));
+                    uint32_t a[4][2];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t word = w[j][4 * k / Codes<SB>::kPerWord];
+                        const int i0 = 4 * k % Codes<SB>::kPerWord;
+                        const float2 x = fma2(make_float2(Codes<SB>::get(word, i0), Codes<SB>::get(word, i0 + 1)), s0, z0);
+                        const float2 y = fma2(make_float2(Codes<SB>::get(word, i0 + 2), Codes<SB>::get(word, i0 + 3)), s1, z1);
+                        a[j][0] = pack_f16(x.x, x.y);
+                        a[j][1] = pack_f16(y.x, y.y);
+                    }
+                    qk(k, a);
                 }
             }
             const int slot0 = item * kGroup;
@@ -304,22 +334,45 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
                     const int at = 4 * (tok * GV + g8 * CN / kGroup);
                     float a = *reinterpret_cast<const float *>(buf + S::VS + at), z = *reinterpret_cast<const float *>(buf + S::VZ + at);
                     if (D == 64 && slot0 + tok < first_slot) a = z = 0.f;
-                    z = fmaf(-BASE, a, z);
+                    if constexpr (!HALF) z = fmaf(-BASE, a, z);
                     sc[t] = make_float2(a, a);
                     ze[t] = make_float2(z, z);
                 }
-#pragma unroll
-                for (int j = 0; j < MT; ++j) {
-                    float2 v[4];  // channels 2j, 2j + 1 of the four tokens
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const uint32_t word = x[t][2 * j / Codes<SB>::kPerWord];
-                        const int i0 = 2 * j % Codes<SB>::kPerWord;
-                        v[t] = fma2(make_float2(Codes<SB>::get(word, i0), Codes<SB>::get(word, i0 + 1)), sc[t], ze[t]);
-                    }
-                    const uint32_t a0 = pack_f16(v[0].x, v[1].x), a1 = pack_f16(v[0].y, v[1].y), a2 = pack_f16(v[2].x, v[3].x), a3 = pack_f16(v[2].y, v[3].y);
+                auto pv = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {  // channels 2j, 2j + 1 of the four tokens
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][j], a0, a1, a2, a3, pb[nt][k][0], pb[nt][k][1]);
+                };
+                if constexpr (HALF) {
+                    // a half of two tokens' words side by side: their codes of a channel are a pair
+                    const uint32_t s01 = pack_f16(sc[0].x, sc[1].x), s23 = pack_f16(sc[2].x, sc[3].x), z01 = pack_f16(ze[0].x, ze[1].x), z23 = pack_f16(ze[2].x, ze[3].x);
+                    constexpr int PER = 16 / SB;  // codes of a half word
+#pragma unroll
+                    for (int j = 0; j < CN; j += PER) {
+                        const uint32_t sel = j / PER % 2 ? 0x7632 : 0x5410;
+                        const uint32_t y01 = __byte_perm(x[0][j / (2 * PER)], x[1][j / (2 * PER)], sel), y23 = __byte_perm(x[2][j / (2 * PER)], x[3][j / (2 * PER)], sel);
+                        uint32_t v01[PER], v23[PER];
+#pragma unroll
+                        for (int i = 0; i < PER; ++i) {
+                            // (2 bits: codes 4-7 of a half lie in its upper byte)
+                            const uint32_t a = SB == 2 && i >= 4 ? y01 >> 8 : y01, b = SB == 2 && i >= 4 ? y23 >> 8 : y23;
+                            v01[i] = hfma2(half_codes<SB>(a, a >> 8, i & 3), s01, z01);
+                            v23[i] = hfma2(half_codes<SB>(b, b >> 8, i & 3), s23, z23);
+                        }
+#pragma unroll
+                        for (int i = 0; i < PER; i += 2) pv((j + i) / 2, v01[i], v01[i + 1], v23[i], v23[i + 1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) {
+                        float2 v[4];
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            const uint32_t word = x[t][2 * j / Codes<SB>::kPerWord];
+                            const int i0 = 2 * j % Codes<SB>::kPerWord;
+                            v[t] = fma2(make_float2(Codes<SB>::get(word, i0), Codes<SB>::get(word, i0 + 1)), sc[t], ze[t]);
+                        }
+                        pv(j, pack_f16(v[0].x, v[1].x), pack_f16(v[0].y, v[1].y), pack_f16(v[2].x, v[3].x), pack_f16(v[2].y, v[3].y));
+                    }
                 }
             }
         } else {
@@ -329,7 +382,10 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
                 lds(a[0], buf + S::row_chunk(tau, c4 * (CH / 8) + i));
                 lds(a[1], buf + S::row_chunk(8 + tau, c4 * (CH / 8) + i));
 #pragma unroll
-                for (int k = 0; k < 4; ++k) { a[0][k] = as_f16x2<T>(a[0][k]); a[1][k] = as_f16x2<T>(a[1][k]); }
+                for (int j = 0; j < 2; ++j) {
+                    const uint4 x = in_order<HALF>(make_uint4(as_f16x2<T>(a[j][0]), as_f16x2<T>(a[j][1]), as_f16x2<T>(a[j][2]), as_f16x2<T>(a[j][3])));
+                    a[j][0] = x.x; a[j][1] = x.y; a[j][2] = x.z; a[j][3] = x.w;
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     mma16816(s[nt][0], a[0][0], a[1][0], a[0][1], a[1][1], qb[nt][4 * i], qb[nt][4 * i + 1]);

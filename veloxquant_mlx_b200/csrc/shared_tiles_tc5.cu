@@ -221,34 +221,16 @@ __device__ __forceinline__ uint4 decode8(const uint32_t (&w)[SB == 8 ? 2 : 1], c
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// The same in half precision, for bfloat16 data and codes of 2 or 4 bits: a code beside the exponent of 1024
-// is the half 1024 + code * 2^bit, one half FMA makes it the code, exactly, and another one the value. Scale and
-// zero are rounded to halves, so a value is off by up to three roundings of 2^-11 instead of one (together
-// less than a quarter of bfloat16's own 2^-8 in the mean), for 13 instructions instead of 20. float16 data
-// keeps the float32 form. Word i of the result holds channels i and i + 4: see in_order.
+// The same in half precision (half_codes). Word i of the result holds channels i and i + 4: see in_order.
 template <int SB>
 __device__ __forceinline__ uint4 decode8_half(uint32_t w, const uint32_t (&sc)[4], const uint32_t (&ze)[4]) {
     uint32_t r[4];
     if constexpr (SB == 2) w = __byte_perm(w, 0u, 0x4140);  // codes 0-3 into the low half, 4-7 into the high one
     const uint32_t w8 = w >> 8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int bit = SB == 2 ? 2 * i : 4 * (i & 1);
-        const uint32_t mask = (SB == 2 ? 0x00030003u : 0x000f000fu) << bit;
-        const uint32_t x = ((SB == 4 && i >= 2 ? w8 : w) & mask) | 0x64006400u;
-        // code = x * 2^-bit - 1024 * 2^-bit
-        const uint32_t down = 0x3c003c00u - (uint32_t)bit * 0x04000400u, off = 0xe400e400u - (uint32_t)bit * 0x04000400u;
-        r[i] = hfma2(hfma2(x, down, off), sc[i], ze[i]);
-    }
+    for (int i = 0; i < 4; ++i) r[i] = hfma2(half_codes<SB>(w, w8, i), sc[i], ze[i]);
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
-// 8 halves in the order in which a tile holds a chunk's channels: as they come, or 0 4 1 5 2 6 3 7
-template <bool SPREAD>
-__device__ __forceinline__ uint4 in_order(uint4 v) {
-    if constexpr (!SPREAD) return v;
-    return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-}
-
 template <int D, int SB, typename T>
 __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __grid_constant__ TileParams p) {
     using L = Layout<D>;
