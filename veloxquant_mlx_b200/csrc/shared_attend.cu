@@ -8,6 +8,7 @@
 // The prefix is read once for all B * H_q/H_kv * S_q query rows of a kv head, the own tokens once per
 // request. Many query rows go to the tcgen05 kernel of shared_tiles_tc5.cu, few to the warp tiles below.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "kivi_attend.h"
@@ -17,7 +18,7 @@ namespace vq {
 namespace {
 
 constexpr int kGroup = 32;
-constexpr int kHalf = 16;   // exact rows of one work item
+constexpr int kExact = 12;  // exact rows of one work item: as many bytes as a packed group of 4-bit codes
 constexpr int kWarps = 4;
 constexpr int kStages = 2;
 
@@ -64,13 +65,13 @@ __device__ __forceinline__ void lds(uint32_t (&w)[N], const uint8_t *p) {
 }
 
 // One stage of a warp's ring: a packed group (key codes | value codes | key scales | key zeros | value
-// scales | value zeros) or 16 exact rows (keys | values).
+// scales | value zeros) or 12 exact rows (keys | values).
 template <int D, int SB>
 struct Stage {
     static constexpr int RB = D * SB / 8, GV = D / kGroup;
     static constexpr int KC = 0, VC = KC + kGroup * RB, KS = VC + kGroup * RB, KZ = KS + 4 * D, VS = KZ + 4 * D, VZ = VS + kGroup * GV * 4;
     static constexpr int PACKED = VZ + kGroup * GV * 4;
-    static constexpr int ROW = 2 * D, VR = kHalf * ROW, EXACT = 2 * kHalf * ROW;
+    static constexpr int ROW = 2 * D, VR = kExact * ROW, EXACT = 2 * kExact * ROW;
     static constexpr int BYTES = PACKED > EXACT ? PACKED : EXACT;
     // Key scales and zeros: the four lanes of a quad read 16-byte chunks that are 128 (64) bytes apart: the
     // chunk's place in its 128-byte line is turned so that they fall on different banks.
@@ -83,14 +84,14 @@ struct Stage {
 // request's own store) over one split of its tokens. Tensor cores by m16n8k16 with tokens (QK^T) and
 // channels (PV) on M and query rows on N: the own part has few rows (H_q/H_kv heads, a few drafted
 // tokens), of which a tcgen05 tile of 128 would waste nearly all.
-// Each warp takes work items in turn (a packed group of 32 tokens, or 16 exact rows), copied by cp.async
+// Each warp takes work items in turn (a packed group of 32 tokens, or 12 exact rows), copied by cp.async
 // into its own two-stage ring, so that an item is in flight while the one before is decoded; no
 // synchronisation between warps until the end. The order of channels and of tokens inside an MMA is
 // free: a lane's K fragments are one run of D/4 channels of a token, its V fragments one run of D/8
 // channels, and the four tokens of a quad lie in rows whose banks differ.
 // Bound by HBM in principle (6 KB a group at 4 bits against about 760 instructions a warp).
 template <int D, int SB, typename T, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
+__global__ void __launch_bounds__(kWarps * 32, NT > 1 ? 2 : SB == 8 ? 3 : 4)
 shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
     using S = Stage<D, SB>;
     constexpr int CH = D / 4, CN = D / 8, KS = D / 16;   // channels a lane owns for K, for V; k-steps of QK^T
@@ -131,8 +132,8 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
     const int n_slots = st.n_quant + st.n_res;
     const int first_slot = is_prefix || !p.own_start ? 0 : min(n_slots, max(0, __ldg(p.own_start + b_own)));
     const int ng = st.n_quant / kGroup;                  // packed items; exact rows start at slot 32 * ng
-    const int items = ng + (st.n_res + kHalf - 1) / kHalf;
-    const int i_first = first_slot < st.n_quant ? first_slot / kGroup : ng + (first_slot - st.n_quant) / kHalf;
+    const int items = ng + (st.n_res + kExact - 1) / kExact;
+    const int i_first = first_slot < st.n_quant ? first_slot / kGroup : ng + (first_slot - st.n_quant) / kExact;
     const int per_split = (items - i_first + ns - 1) / ns;
     const int i_lo = min(items, i_first + split * per_split), i_hi = min(items, i_lo + per_split);
 
@@ -167,9 +168,9 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
                 copy16(dst + S::VZ + 16 * lane, vz + slot0 * GV + 4 * lane, live);
             }
         } else {
-            const int r0 = (item - ng) * kHalf;
+            const int r0 = (item - ng) * kExact;
 #pragma unroll
-            for (int j = lane; j < kHalf * (D / 8); j += 32) {
+            for (int j = lane; j < kExact * (D / 8); j += 32) {
                 const int r = j / (D / 8), ch = j % (D / 8);
                 const bool in = r0 + r < st.n_res, seen = in && st.n_quant + r0 + r >= first_slot;
                 const int64_t at = in ? (int64_t)(r0 + r) * D + 8 * ch : 0;
@@ -214,6 +215,7 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
     // Returns the weights as B fragments of the item's 16-token steps.
     auto softmax = [&](auto steps_c, float (&s)[NT][2][4], int slot0, uint32_t (&pb)[NT][2][2]) {
         constexpr int STEPS = decltype(steps_c)::value;
+        const int end = STEPS == 1 ? slot0 + kExact : INT_MAX;  // (the last rows of an exact tile are not there)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float mx[2] = {-INFINITY, -INFINITY};
@@ -222,7 +224,7 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const int slot = slot0 + 16 * k + 8 * (c >> 1) + tau;
-                    s[nt][k][c] = slot >= first_slot && slot < lim[nt][c & 1] ? s[nt][k][c] * p.scale_log2 : -INFINITY;
+                    s[nt][k][c] = slot >= first_slot && slot < min(lim[nt][c & 1], end) ? s[nt][k][c] * p.scale_log2 : -INFINITY;
                     mx[c & 1] = fmaxf(mx[c & 1], s[nt][k][c]);
                 }
             float base[2], f[2];
@@ -380,7 +382,7 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
             for (int i = 0; i < CH / 8; ++i) {
                 uint32_t a[2][4];
                 lds(a[0], buf + S::row_chunk(tau, c4 * (CH / 8) + i));
-                lds(a[1], buf + S::row_chunk(8 + tau, c4 * (CH / 8) + i));
+                lds(a[1], buf + S::row_chunk(min(8 + tau, kExact - 1), c4 * (CH / 8) + i));
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const uint4 x = in_order<HALF>(make_uint4(as_f16x2<T>(a[j][0]), as_f16x2<T>(a[j][1]), as_f16x2<T>(a[j][2]), as_f16x2<T>(a[j][3])));
@@ -392,12 +394,12 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
                     mma16816(s[nt][0], a[0][2], a[1][2], a[0][3], a[1][3], qb[nt][4 * i + 2], qb[nt][4 * i + 3]);
                 }
             }
-            softmax(std::integral_constant<int, 1>{}, s, st.n_quant + (item - ng) * kHalf, pb);
+            softmax(std::integral_constant<int, 1>{}, s, st.n_quant + (item - ng) * kExact, pb);
 #pragma unroll
             for (int i = 0; i < CN / 8; ++i) {
-                uint32_t x[4][4];
+                uint32_t x[kExact / 4][4];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
+                for (int t = 0; t < kExact / 4; ++t) {
                     lds(x[t], buf + S::VR + S::row_chunk(4 * t + c4, g8 * (CN / 8) + i));
 #pragma unroll
                     for (int k = 0; k < 4; ++k) x[t][k] = as_f16x2<T>(x[t][k]);
@@ -405,7 +407,7 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t a0 = __byte_perm(x[0][j], x[1][j], 0x5410), a1 = __byte_perm(x[0][j], x[1][j], 0x7632);
-                    const uint32_t a2 = __byte_perm(x[2][j], x[3][j], 0x5410), a3 = __byte_perm(x[2][j], x[3][j], 0x7632);
+                    const uint32_t a2 = x[2][j] & 0xffffu, a3 = x[2][j] >> 16;  // (rows 12 to 15 are zero)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][4 * i + j], a0, a1, a2, a3, pb[nt][0][0], pb[nt][0][1]);
                 }
@@ -542,7 +544,7 @@ int32_t plan_of(const vq_shared_attend_args &a, const DeviceInfo &di, Plan *out)
     const int64_t per_req = (int64_t)(a.H_q / a.H_kv) * a.S_q, all = a.B * per_req;
     pl.rows = (int64_t)a.B * a.H_q * a.S_q;
     const vq_kivi_rows &pre = a.prefix, &own = a.own;
-    const int ip = pre.n_quant / kGroup + (int)ceil_div(pre.n_res, kHalf), io = own.n_quant / kGroup + (int)ceil_div(own.n_res, kHalf);
+    const int ip = pre.n_quant / kGroup + (int)ceil_div(pre.n_res, kExact), io = own.n_quant / kGroup + (int)ceil_div(own.n_res, kExact);
     // The tcgen05 kernel decodes a token once for 128 or 256 query rows, the warp tiles for 8 or 16: it
     // pays from two of the wider ones on (33 rows behind 2K tokens: 12 against 14 us), but not for a prefix
     // of a few hundred tokens, where its setup shows. It takes scales that are not negative.
@@ -555,8 +557,8 @@ int32_t plan_of(const vq_shared_attend_args &a, const DeviceInfo &di, Plan *out)
     pl.prefix_tiles = (int)ceil_div(all, pl.row_tile);
     pl.own_tiles = (int)ceil_div(per_req, pl.row_tile);
     auto splits = [&](int64_t units, int items) {
-        // enough CTAs to fill the GPU, but at least two work items a warp
-        return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div((int64_t)di.sm_count * 3, units), ceil_div(items, 2 * kWarps), 64}));
+        // as many CTAs as fit the GPU at once, but at least two work items a warp (32K: 1 split 22 us, 2 28 us)
+        return (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)di.sm_count * 4 / units, ceil_div(items, 2 * kWarps), 64}));
     };
     pl.np = !ip ? 0 : pl.prefix_tc5 ? shared_tiles_tc5_records(all, pl.prefix_tc5) : a.n_splits > 0 ? std::min({a.n_splits, ip, 64})
                                                                                                    : splits((int64_t)a.H_kv * pl.prefix_tiles, ip);
