@@ -240,3 +240,79 @@ def test_cache_update_rotary_equals_rotating_first(b):
         assert torch.equal(q1, q2) and one.offset == two.offset == n and one._n_res == two._n_res and one._n_quantized == two._n_quantized
         assert torch.equal(one.fused_sdpa(q1[:, :, -1:].contiguous(), 0.09), two.fused_sdpa(q2[:, :, -1:].contiguous(), 0.09))
     assert all(torch.equal(x, y) for x, y in zip(one.state, two.state))
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements, in the tokens of one head and in the rows behind which an append goes."""
+    S = (1 << 24) + 5
+    x = torch.empty(1, 1, S, 136, dtype=BF, device=DEV)[..., :128]  # 2.3e9 elements apart
+    tail = _rand((1, 1, 9, 128), BF, 40)
+    x[:, :, -9:] = tail
+    rope = RotaryEmbedding(128, rotary_dim=64)
+    y = rope(x, positions=7)[:, :, -9:]
+    pos = 7 + S - 9 + torch.arange(9, device=DEV)[None]
+    _close(y, *_turn64(tail, rope.inv_freq, pos, "half", 64))
+    assert torch.equal(y[..., 64:], tail[..., 64:])
+    del x, y
+    rows = (1 << 24) + 100
+    res = torch.zeros(2, 1, 1, rows, 132, dtype=BF, device=DEV)[..., :128]
+    q, k, v = (_rand((1, 1, 3, 128), BF, 41 + i) for i in range(3))
+    rope.append(q, k, v, res[0], res[1], rows - 3, 5)
+    _close(res[0, :, :, -3:], *_turn64(k, rope.inv_freq, 5 + torch.arange(3, device=DEV)[None], "half", 64))
+    assert torch.equal(res[1, :, :, -3:], v) and not res[:, :, :, :1000].any() and not res[:, :, :, -200:-3].any()
+
+
+def test_forward_and_gradient_inside_a_graph():
+    rope = RotaryEmbedding(64, device=DEV)
+    q, k = _rand((2, 4, 3, 64), F, 50).requires_grad_(True), _rand((2, 2, 3, 64), F, 51).requires_grad_(True)
+    pos = torch.randint(0, 99, (2, 3), device=DEV)
+    gq, gk = _rand((2, 4, 3, 64), F, 52), _rand((2, 2, 3, 64), F, 53)
+
+    def step():
+        yq, yk = rope(q, k, pos)
+        return (yq, yk, *torch.autograd.grad((yq, yk), (q, k), (gq, gk)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    with torch.no_grad():
+        q.mul_(3)
+        gk.add_(1)
+    pos.add_(100)
+    g.replay()
+    assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+def test_the_same_tensor_twice_and_a_half_used_pair():
+    rope = RotaryEmbedding(64)
+    q = _rand((1, 2, 5, 64), F, 60).requires_grad_(True)
+    a, b = rope(q, q, 3)
+    assert torch.equal(a, b)
+    (d,) = torch.autograd.grad((a, b), q, (torch.ones_like(a), torch.ones_like(b)))
+    want, mag = _turn64(torch.ones_like(q), rope.inv_freq, 3 + torch.arange(5, device=DEV)[None], "half", 64, 1.0, -1.0)
+    _close(d, 2 * want, 2 * mag)
+    with torch.no_grad():
+        assert not rope(q)[0].requires_grad
+
+
+def test_update_rotary_of_a_cache_with_its_own_append():
+    """kivi_sink replaces update_and_fetch: it gets rotated keys through it."""
+    from veloxquant_mlx_b200.cache import KVCacheConfig, KVCacheFactory
+
+    def make():
+        return KVCacheFactory.create(KVCacheConfig(method="kivi_sink", head_dim=128, bit_width_inlier=4, residual_length=32, n_sink_tokens=2))
+
+    rope, one, two = RotaryEmbedding(128), make(), make()
+    n = 0
+    for S in (50, 1, 1):
+        q, k, v = (_rand((1, h, S, 128), HF, 70 + S + h) for h in (4, 2, 2))
+        q1, k1, v1 = one.update_rotary(q, k, v, rope)
+        q2, k2 = rope(q, k, n)
+        k3, v3 = two.update_and_fetch(k2, v)
+        n += S
+        assert torch.equal(q1, q2) and torch.equal(k1, k3) and torch.equal(v1, v3)

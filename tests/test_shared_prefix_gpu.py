@@ -364,3 +364,50 @@ def test_a_fork_of_a_transformers_cache_continues_a_prompt():
                 assert fork.get_seq_length() == 94
                 # 8-bit codes of the same tokens; the alone cache packs a group that the fork still holds exactly
                 assert (got.float() - together[i][b].float()).abs().max() < 0.05 * got.float().abs().max() + 0.05
+
+
+def test_exact_rows_past_32_bits():
+    rows, D = (1 << 24) + 64, 128  # 2.1e9 elements a slab; the second request's begin behind it
+    k = torch.empty(2, 1, rows, D, dtype=HF, device=DEV)
+    v = torch.empty(2, 1, rows, D, dtype=HF, device=DEV)
+    small = [torch.randn(2, 1, 40, D, device=DEV, generator=_gen(50 + i)).half() for i in range(2)]
+    k[:, :, -50:-10], v[:, :, -50:-10] = small
+    own = KiviRows(k_res=k, v_res=v, n_res=40, res_offset=rows - 50)
+    dense = []
+    for t in small:
+        dense += [t.double(), torch.zeros_like(t, dtype=torch.float64)]
+    pre = make_store(1, 1, D, 4, 64, 3, HF, 52)
+    for S in (1, 36):
+        q = torch.randn(2, 2, S, D, device=DEV, generator=_gen(53)).half()
+        check(q, pre, (own, dense), D**-0.5)
+        check(q, pre, (own, dense), D**-0.5, variant=2)
+
+
+@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_constant_groups_and_large_offsets(variant, dtype):
+    """Groups without spread (scale at its floor) and keys far from zero: code * scale + zero must not lose the zero."""
+    B, H, D = 40, 1, 128
+    k = (100 + torch.randn(1, H, 256, D, device=DEV, generator=_gen(60))).to(dtype)
+    k[:, :, :32] = 3.0
+    v = (-50 + torch.randn(1, H, 256, D, device=DEV, generator=_gen(61))).to(dtype)
+    v[:, :, 40:50] = 7.0
+    t = {}
+    t["k_codes"], t["k_scale"], t["k_zero"] = kernels.kivi_quantize(k, -2, 32, 4)
+    t["v_codes"], t["v_scale"], t["v_zero"] = kernels.kivi_quantize(v, -1, 32, 4)
+    q = 0.05 * torch.randn(B, 1, 1, D, device=DEV, generator=_gen(62)).to(dtype)
+    check(q, (KiviRows(**t), dense_of(t, 4, 256, D, 1, H)), None, 0.1, variant=variant)
+
+
+def test_a_nan_that_is_seen_stays_in_its_rows():
+    q = torch.randn(40, 2, 1, 128, device=DEV, generator=_gen(70)).half()
+    q[3, 1] = float("nan")
+    pre, own = make_store(1, 1, 128, 4, 512, 9, HF, 71), make_store(40, 1, 128, 4, 32, 5, HF, 72)
+    own[0]._tensors[7][9, 0, 2, 5] = float("nan")  # a value of request 9
+    for variant in (1, 2):
+        out = kivi_shared_prefix_attend(q, pre[0], own[0], 0.1, variant=variant)
+        bad = out.isnan()
+        assert bool(bad[3, 1].all()) and bool(bad[9, :, :, 5].all())
+        bad[3, 1] = False
+        bad[9, :, :, 5] = False
+        assert not bool(bad.any())

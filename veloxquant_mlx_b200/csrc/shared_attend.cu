@@ -206,6 +206,14 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
         }
     }
 
+    int all_see = INT_MAX;  // slots that every live row sees need no mask
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (tile * ROWS + 8 * nt + 2 * c4 + i < n_rows) all_see = min(all_see, lim[nt][i]);
+    all_see = __reduce_min_sync(0xffffffffu, all_see);
+
     float o[NT][MT][4] = {};
     float m[NT][2], l[NT][2];
 #pragma unroll
@@ -216,17 +224,28 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
     auto softmax = [&](auto steps_c, float (&s)[NT][2][4], int slot0, uint32_t (&pb)[NT][2][2]) {
         constexpr int STEPS = decltype(steps_c)::value;
         const int end = STEPS == 1 ? slot0 + kExact : INT_MAX;  // (the last rows of an exact tile are not there)
+        const bool all_seen = STEPS == 2 && slot0 >= first_slot && slot0 + kGroup <= all_see;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float mx[2] = {-INFINITY, -INFINITY};
+            if (all_seen) {
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k)
+                for (int k = 0; k < STEPS; ++k)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int slot = slot0 + 16 * k + 8 * (c >> 1) + tau;
-                    s[nt][k][c] = slot >= first_slot && slot < min(lim[nt][c & 1], end) ? s[nt][k][c] * p.scale_log2 : -INFINITY;
-                    mx[c & 1] = fmaxf(mx[c & 1], s[nt][k][c]);
-                }
+                    for (int c = 0; c < 4; ++c) {
+                        s[nt][k][c] *= p.scale_log2;
+                        mx[c & 1] = fmaxf(mx[c & 1], s[nt][k][c]);
+                    }
+            } else {
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int slot = slot0 + 16 * k + 8 * (c >> 1) + tau;
+                        s[nt][k][c] = slot >= first_slot && slot < min(lim[nt][c & 1], end) ? s[nt][k][c] * p.scale_log2 : -INFINITY;
+                        mx[c & 1] = fmaxf(mx[c & 1], s[nt][k][c]);
+                    }
+            }
             float base[2], f[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -469,14 +488,15 @@ int32_t launch_rows(const RowsParams &p, unsigned blocks, bool dependent, cudaSt
 
 // Joins the records of an output row: `ways` warps (1 or 4) take its records in turn, each lane D/32
 // channels; every warp has all of the row's (m, l) in its lanes. Bound by latency (a few KB a row, from
-// L2), so eight records are requested at a time.
+// L2), so eight records are asked for at a time, the first eight together with the (m, l).
 constexpr int kMaxRecords = 128;  // 64 splits of either part
 
 template <int D, typename T>
 __global__ void __launch_bounds__(128) shared_attend_merge_kernel(const SharedPartials parts, int64_t rows, int ways, T *__restrict__ out, float *__restrict__ lse) {
-    constexpr int C = D / 32;
+    constexpr int C = D / 32, AHEAD = 8;
     using V = typename std::conditional<C == 4, float4, float2>::type;
     __shared__ float sh[4][D];
+    __shared__ float sh_w[4][kMaxRecords];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int part = warp % ways;
     const int64_t row = (int64_t)blockIdx.x * (4 / ways) + warp / ways;
@@ -485,6 +505,11 @@ __global__ void __launch_bounds__(128) shared_attend_merge_kernel(const SharedPa
     wait_for_previous();
     if (row < rows) {
         const float2 *ml = reinterpret_cast<const float2 *>(parts.ml) + row * n;
+        const V *po = reinterpret_cast<const V *>(parts.o + row * n * D) + lane;
+        V v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (part + i * ways < n) v[i] = po[(int64_t)(part + i * ways) * 32];
         float2 r[kMaxRecords / 32];
 #pragma unroll
         for (int i = 0; i < kMaxRecords / 32; ++i) {
@@ -495,22 +520,26 @@ __global__ void __launch_bounds__(128) shared_attend_merge_kernel(const SharedPa
         const float bs = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
         for (int i = 0; i < kMaxRecords / 32; ++i) {
-            r[i].x = ex2(r[i].x - bs);  // the record's weight
-            ll = fmaf(r[i].y, r[i].x, ll);
+            const float f = ex2(r[i].x - bs);  // the record's weight
+            ll = fmaf(r[i].y, f, ll);
+            sh_w[warp][32 * i + lane] = f;
         }
         ll = warp_sum(ll);
-        const V *po = reinterpret_cast<const V *>(parts.o + row * n * D) + lane;
+        __syncwarp();
+        for (int j0 = part;; ) {
 #pragma unroll
-        for (int i = 0; i < kMaxRecords / 32; ++i) {
-            const int last = min(32, n - 32 * i);
-#pragma unroll 8
-            for (int j = part; j < last; j += ways) {
-                const V v = po[(int64_t)(32 * i + j) * 32];
-                const float f = __shfl_sync(0xffffffffu, r[i].x, j);
-                const float *e = reinterpret_cast<const float *>(&v);
+            for (int i = 0; i < AHEAD; ++i) {
+                if (j0 + i * ways >= n) break;
+                const float f = sh_w[warp][j0 + i * ways];
+                const float *e = reinterpret_cast<const float *>(&v[i]);
 #pragma unroll
                 for (int c = 0; c < C; ++c) acc[c] = fmaf(e[c], f, acc[c]);
             }
+            j0 += AHEAD * ways;
+            if (j0 >= n) break;
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                if (j0 + i * ways < n) v[i] = po[(int64_t)(j0 + i * ways) * 32];
         }
     }
     if (ways > 1) {
@@ -545,24 +574,33 @@ int32_t plan_of(const vq_shared_attend_args &a, const DeviceInfo &di, Plan *out)
     pl.rows = (int64_t)a.B * a.H_q * a.S_q;
     const vq_kivi_rows &pre = a.prefix, &own = a.own;
     const int ip = pre.n_quant / kGroup + (int)ceil_div(pre.n_res, kExact), io = own.n_quant / kGroup + (int)ceil_div(own.n_res, kExact);
-    // The tcgen05 kernel decodes a token once for 128 or 256 query rows, the warp tiles for 8 or 16: it
-    // pays from two of the wider ones on (33 rows behind 2K tokens: 12 against 14 us), but not for a prefix
-    // of a few hundred tokens, where its setup shows. It takes scales that are not negative.
+    // The tcgen05 kernel decodes a token once for 128 or 256 query rows, the warp tiles for 8 or 16, but it
+    // takes 5 us longer to start and end. Measured with 8 kv heads, warp tiles / tcgen05 in us: 64 rows
+    // behind 1K tokens 10.4 / 12.6, 2K 14.1 / 13.3, 8K 29 / 19; 32 rows behind 2K 9.7 / 12.7, 8K 19.9 / 18.3;
+    // 16 rows behind 32K 27.6 / 32.2; own tokens, 1 request of 128 rows over 662: 14.6 / 18.5, of 256: 21.8 /
+    // 17.2; 8 of 36 over 100: 14.3 / 15.4, over 662: 26.6 / 23.0. It takes scales that are not negative.
+    auto pays = [&](int64_t units, int64_t rows, const vq_kivi_rows &st) {
+        return rows >= 32 && (double)units * (double)rows * ((double)st.n_quant + st.n_res) >= 1 << 20;
+    };
     const bool can = a.scale >= 0.f;
     VQ_REQUIRE(a.variant != 2 || (can && ip), VQ_ERR_SHAPE, "vq_kivi_shared_attend: the tcgen05 kernel needs a prefix and a scale that is not negative");
-    if (can && ip && (a.variant == 2 || (a.variant == 0 && all > 2 * 16 && (int64_t)pre.n_quant + pre.n_res >= 512)))
-        pl.prefix_tc5 = shared_tiles_tc5_splits(pre, a.H_kv, all, a.n_splits, di);
-    if (can && io && a.variant != 1 && per_req > 2 * 16) pl.own_tc5 = shared_tiles_tc5_splits(own, (int64_t)a.B * a.H_kv, per_req, 0, di);
+    if (can && ip && (a.variant == 2 || (a.variant == 0 && pays(a.H_kv, all, pre))))
+        pl.prefix_tc5 = shared_tiles_tc5_splits(pre, a.H_kv, all, a.D, a.n_splits, di);
+    const int64_t units = (int64_t)a.B * a.H_kv;
+    if (can && io && (a.variant == 2 ? per_req > 32 : a.variant == 0 && pays(units, per_req, own)))
+        pl.own_tc5 = shared_tiles_tc5_splits(own, units, per_req, a.D, 0, di);
     pl.row_tile = (pl.prefix_tc5 ? per_req : all) > 8 ? 16 : 8;
     pl.prefix_tiles = (int)ceil_div(all, pl.row_tile);
     pl.own_tiles = (int)ceil_div(per_req, pl.row_tile);
-    auto splits = [&](int64_t units, int items) {
-        // as many CTAs as fit the GPU at once, but at least two work items a warp (32K: 1 split 22 us, 2 28 us)
-        return (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)di.sm_count * 4 / units, ceil_div(items, 2 * kWarps), 64}));
+    auto splits = [&](int64_t tiles, int items) {
+        // as many CTAs as fit the GPU at once, but at least two work items a warp (512 units of 26 items:
+        // 1 split 25 us, 2 28 us, 4 33 us)
+        return (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)di.sm_count * 4 / tiles, ceil_div(items, 2 * kWarps), 64}));
     };
-    pl.np = !ip ? 0 : pl.prefix_tc5 ? shared_tiles_tc5_records(all, pl.prefix_tc5) : a.n_splits > 0 ? std::min({a.n_splits, ip, 64})
-                                                                                                   : splits((int64_t)a.H_kv * pl.prefix_tiles, ip);
-    pl.no = !io ? 0 : pl.own_tc5 ? shared_tiles_tc5_records(per_req, pl.own_tc5) : splits((int64_t)a.B * a.H_kv * pl.own_tiles, io);
+    if (pl.prefix_tc5) pl.np = shared_tiles_tc5_records(all, pl.prefix_tc5);
+    else if (ip) pl.np = a.n_splits > 0 ? std::min({a.n_splits, ip, 64}) : splits((int64_t)a.H_kv * pl.prefix_tiles, ip);
+    if (pl.own_tc5) pl.no = shared_tiles_tc5_records(per_req, pl.own_tc5);
+    else if (io) pl.no = splits(units * pl.own_tiles, io);
     *out = pl;
     return VQ_OK;
 }
@@ -584,7 +622,7 @@ int32_t validate(const vq_shared_attend_args &a) {
         const char *which = s == &a.prefix ? "prefix" : "own";
         VQ_REQUIRE(s->n_quant >= 0 && s->n_res >= 0 && s->n_quant % kGroup == 0, VQ_ERR_SHAPE, "%s: %s: n_quant=%d must be a multiple of 32 and n_res=%d not negative",
                    fn, which, s->n_quant, s->n_res);
-        VQ_REQUIRE((int64_t)s->n_quant + s->n_res < (1ll << 31) - 64, VQ_ERR_SHAPE, "%s: %s: too many tokens", fn, which);
+        VQ_REQUIRE((int64_t)s->n_quant + s->n_res < (1ll << 31) - 256, VQ_ERR_SHAPE, "%s: %s: too many tokens", fn, which);
         if (s->n_quant) {
             VQ_REQUIRE(s->k_codes && s->v_codes && s->k_scale && s->k_zero && s->v_scale && s->v_zero, VQ_ERR_SHAPE, "%s: %s: a packed tensor is NULL", fn, which);
             VQ_REQUIRE(is_aligned(s->k_codes, 16) && is_aligned(s->v_codes, 16) && is_aligned(s->k_scale, 16) && is_aligned(s->k_zero, 16) &&
@@ -647,7 +685,7 @@ int32_t launch_all(const vq_shared_attend_args &a, const Plan &pl, const DeviceI
 
 extern "C" int64_t vq_kivi_shared_attend_workspace_bytes(const vq_shared_attend_args *args) {
     using namespace vq;
-    if (!args || args->H_kv < 1 || args->H_q % args->H_kv || args->B < 1 || args->S_q < 1) return 0;
+    if (!args || validate(*args) != VQ_OK) return 0;
     DeviceInfo di;
     if (device_info(&di) != VQ_OK) { di.sm_count = 148; di.smem_optin = 227 * 1024; }
     Plan pl;

@@ -18,7 +18,7 @@ struct SharedPartials {
 // rows; its launch for the prefix (prefix_splits > 0, records from 0) and the own tokens (own_splits > 0,
 // records from own_record0); its "a bounded wait gave up" flag. A part of at most 128 rows a unit leaves two
 // records per split.
-int shared_tiles_tc5_splits(const vq_kivi_rows &st, int64_t units, int64_t rows, int wanted, const DeviceInfo &di);
+int shared_tiles_tc5_splits(const vq_kivi_rows &st, int64_t units, int64_t rows, int D, int wanted, const DeviceInfo &di);
 inline int shared_tiles_tc5_records(int64_t rows, int splits) { return rows > 128 ? splits : 2 * splits; }
 int32_t shared_tiles_tc5_launch(const vq_shared_attend_args &a, const SharedPartials &parts, int prefix_splits, int own_splits, int own_record0,
                                 cudaStream_t stream);

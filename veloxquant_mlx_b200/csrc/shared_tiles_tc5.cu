@@ -701,20 +701,21 @@ int32_t launch_bits(int sb, const TileParams &p, unsigned blocks, cudaStream_t s
 
 }  // namespace
 
-// Splits of one part along its tokens. The time of a split count, in token tiles: waves of CTAs (one an
-// SM) times the longest CTA (its tiles and a fixed part for setup and epilogue), plus the merge's
-// reading of the records.
-int shared_tiles_tc5_splits(const vq_kivi_rows &st, int64_t units, int64_t rows, int wanted, const DeviceInfo &di) {
+// Splits of one part along its tokens: the count with the smallest estimate in microseconds. A wave of CTAs
+// (one an SM) takes 8 for setup and epilogue and 2.5 (head_dim 64: 2) a token tile with two row tiles, or a
+// pair of token tiles with one; a partial record of a row costs 0.2 ns more (written here, read by the
+// merge). Measured at 16 requests behind 8K tokens: 6 splits 26.8, 10 22.3, 18 23.4; 96 requests behind 4K,
+// head_dim 64: 6 23.1, 11 19.6, 18 22.4; 64 requests behind 32K: 12 84.2, 18 71.8.
+int shared_tiles_tc5_splits(const vq_kivi_rows &st, int64_t units, int64_t rows, int D, int wanted, const DeviceInfo &di) {
     const int tiles = tiles_of(st), most = std::min(tiles, 32);
     if (wanted > 0) return std::min(wanted, most);
     const int64_t ctas = units * row_blocks_of(rows);
-    const int rt = rows > kTile ? 2 : 1;
     int best = 1;
-    double cheapest = 1e30;
+    double least = 1e30;
     for (int s = 1; s <= most; ++s) {
-        const double waves = (double)ceil_div(ctas * s, di.sm_count);
-        const double t = waves * ((double)ceil_div(tiles, s) + 3.0) + 0.02 * s * (double)ceil_div(ctas * rt * s, di.sm_count);
-        if (t < cheapest) { cheapest = t; best = s; }
+        const int64_t longest = ceil_div(tiles, s), steps = rows > kTile ? longest : ceil_div(longest, 2);
+        const double us = (double)ceil_div(ctas * s, di.sm_count) * (8.0 + (D == 128 ? 2.5 : 2.0) * (double)steps) + 2e-4 * 2 * kTile * (double)(ctas * s);
+        if (us < least) { least = us; best = s; }
     }
     return best;
 }

@@ -17,10 +17,11 @@ from typing import Any
 import torch
 
 from . import _lib
-from ._lib import ROTARY_PACK, check, dtype_code, lib, require_cuda, stream_ptr
+from ._lib import _DTYPE_CODE as _DTYPE_CODES
+from ._lib import ROTARY_PACK, check, lib, require_cuda, stream_ptr
 
 _LAYOUTS = ("half", "interleaved")
-_NONE = (0, 0, 0, 0)
+_NO_STRIDE = (0, 0, 0)
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
@@ -204,16 +205,32 @@ class RotaryEmbedding:
         pos, psb, pss, off = self._positions(fn, positions, B, S, dev)
         x0, x1, x2, _ = q.stride()
         y0, y1, y2, _ = q_out.stride()
-        k0, k1, k2, _ = k.stride() if k is not None else _NONE
-        v0, v1, v2, _ = v.stride() if v is not None else _NONE
+        if k is None:
+            k_ptr = Hk = k0 = k1 = k2 = 0
+        else:
+            k_ptr, Hk = k.data_ptr(), k.shape[1]
+            k0, k1, k2, _ = k.stride()
+        if v is None:
+            v_ptr = Hv = v0 = v1 = v2 = 0
+        else:
+            v_ptr, Hv = v.data_ptr(), v.shape[1]
+            v0, v1, v2, _ = v.stride()
+        if pos is None:
+            pos_ptr, pos_bytes = 0, 8
+        else:
+            pos_ptr, pos_bytes = pos.data_ptr(), 8 if pos.dtype is torch.int64 else 4
         a = ROTARY_PACK.pack(
-            q.data_ptr(), 0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(), q_out.data_ptr(), k_out, v_out,
-            x0, x1, x2, k0, k1, k2, v0, v1, v2, y0, y1, y2, *k_out_stride, *v_out_stride,
-            Hq, 0 if k is None else k.shape[1], 0 if v is None else v.shape[1], dtype_code(q.dtype), B, S, D, self.rotary_dim,
-            self._layout_code, 1 if inverse else 0, 0 if pos is None else pos.data_ptr(), 8 if pos is None else pos.element_size(),
+            q.data_ptr(), k_ptr, v_ptr, q_out.data_ptr(), k_out, v_out, x0, x1, x2, k0, k1, k2, v0, v1, v2, y0, y1, y2, *k_out_stride, *v_out_stride,
+            Hq, Hk, Hv, _DTYPE_CODES[q.dtype], B, S, D, self.rotary_dim, self._layout_code, 1 if inverse else 0, pos_ptr, pos_bytes,
             self.attention_factor, psb, pss, off, self._turns_on(dev))
-        with _lib.on_device(dev):
-            check(lib().vq_rotary(a, stream_ptr(dev)), fn)
+        native = lib()
+        if dev.index == torch.cuda.current_device():  # (the usual case, without a context manager)
+            status = native.vq_rotary(a, stream_ptr(dev))
+        else:
+            with _lib.on_device(dev):
+                status = native.vq_rotary(a, stream_ptr(dev))
+        if status:
+            check(status, fn)
 
     # -- calls ---------------------------------------------------------------------------
     def __call__(self, q: torch.Tensor, k: torch.Tensor | None = None, positions=None, *, inverse: bool = False):
@@ -231,12 +248,12 @@ class RotaryEmbedding:
             q = q.contiguous()
         yq = _empty(q)
         if k is None:
-            self._launch(fn, q, yq, None, 0, _NONE[:3], None, 0, _NONE[:3], positions, inverse)
+            self._launch(fn, q, yq, None, 0, _NO_STRIDE, None, 0, _NO_STRIDE, positions, inverse)
             return yq, None
         if k.stride(3) != 1:
             k = k.contiguous()
         yk = _empty(k)
-        self._launch(fn, q, yq, k, yk.data_ptr(), yk.stride()[:3], None, 0, _NONE[:3], positions, inverse)
+        self._launch(fn, q, yq, k, yk.data_ptr(), yk.stride()[:3], None, 0, _NO_STRIDE, positions, inverse)
         return yq, yk
 
     def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_res: torch.Tensor, v_res: torch.Tensor, tok_offset: int,
