@@ -109,12 +109,14 @@ class RotaryEmbedding:
     contiguous tensors: ``q [B, H_q, S, D]``, ``k [B, H_kv, S, D]`` in float16, bfloat16 or float32
     with any strides (heads in the projection's ``[B, S, H, D]`` order included). ``positions`` is an
     integer tensor ``[S]``, ``[1, S]`` or ``[B, S]`` on the same device, or an int: the position of token
-    0, the others following. ``inverse=True`` turns back. Products are float32, angles float64 (exact
+    0, the others following (default 0). ``inverse=True`` turns the other way, times the same
+    ``attention_factor``: the gradient. Products are float32, angles float64 (exact
     to float32 for positions up to 2**31 and beyond); one rounding to the tensors' type at the end.
     Gradients flow to ``q`` and ``k`` (also twice), not to positions or frequencies.
 
     The frequency table is put on a device at its first use there; make that use (or pass
-    ``device=``) before a CUDA-graph capture.
+    ``device=``) before a CUDA-graph capture. Where a backward pass is captured, PyTorch's own rule
+    holds: no graph that an earlier eager pass built over the same leaves may still be alive.
     """
 
     def __init__(self, head_dim: int, *, rotary_dim: int | None = None, base: float = 10000.0, layout: str = "half",
@@ -129,17 +131,23 @@ class RotaryEmbedding:
         else:
             if scaling is not None:
                 raise ValueError("RotaryEmbedding: give inv_freq or scaling, not both")
-            freq, factor = torch.as_tensor(inv_freq).detach().to("cpu", torch.float64), 1.0
+            freq, factor = torch.as_tensor(inv_freq).detach().double(), 1.0
             if tuple(freq.shape) != (rotary_dim // 2,):
                 raise ValueError(f"RotaryEmbedding: inv_freq must have shape ({rotary_dim // 2},), got {tuple(freq.shape)}")
         self.head_dim, self.rotary_dim, self.layout = int(head_dim), rotary_dim, layout
         self._layout_code = _LAYOUTS.index(layout)
-        self.inv_freq = freq
+        self._freq = freq  # (float64, where it was given)
         self.attention_factor = float(factor if attention_factor is None else attention_factor)
-        self._turns_host = freq / (2.0 * math.pi)
-        self._turns: dict = {}
+        self._turns: dict = {}  # device index -> turns per position of each pair
+        if device is None and freq.is_cuda:
+            device = freq.device
         if device is not None:
             self._turns_on(torch.device(device))
+
+    @property
+    def inv_freq(self) -> torch.Tensor:
+        """Angle per position of each pair, float64 on the host."""
+        return self._freq.cpu()
 
     def _turns_on(self, device: torch.device) -> int:
         """The table's address on ``device``."""
@@ -148,8 +156,8 @@ class RotaryEmbedding:
         if t is None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("RotaryEmbedding: first use on a device inside a graph capture; pass device= or call it once before")
-            with _lib.on_device(device):
-                t = self._turns_host.to(torch.device("cuda", index))
+            with _lib.on_device(torch.device("cuda", index)):
+                t = self._freq.to(torch.device("cuda", index)) / (2.0 * math.pi)
                 torch.cuda.current_stream().synchronize()  # (any stream may read it from here on)
             self._turns[index] = t
         return t.data_ptr()
