@@ -61,8 +61,10 @@ typedef enum vq_knob {
                                     bounded wait runs out, the kernel finishes normally and
                                     vq_kivi_attend_status reports VQ_ERR_TIMEOUT once (one-shot
                                     self-test of that path; nothing faults or hangs) */
-    VQ_KNOB_VQ_WAIT_TEST = 4     /* 1: the same for the NEXT tcgen05 vq_vq_quantize launch and
+    VQ_KNOB_VQ_WAIT_TEST = 4,    /* 1: the same for the NEXT tcgen05 vq_vq_quantize launch and
                                     vq_vq_quantize_status */
+    VQ_KNOB_SHARED_WAIT_TEST = 5 /* 1: the same for the NEXT tcgen05 launch of vq_kivi_shared_attend
+                                    and vq_kivi_attend_status */
 } vq_knob;
 int32_t vq_tune(int32_t knob, int32_t value);
 
@@ -624,8 +626,8 @@ typedef struct vq_kivi_rows {
  * `own`) is seen by query row r when t >= own_start[b] (NULL: 0; slots before it are padding) and,
  * with VQ_ATTEND_CAUSAL, t <= n - S_q + r. A row that sees nothing gives zeros (and lse -inf).
  * float16 or bfloat16; D 64 or 128, group 32, store_bits 2, 4 or 8. Decoded keys and values
- * enter the tensor cores as float16 (also for bfloat16 queries), so code*scale+zero, the exact
- * rows and q must lie within +-65504. */
+ * enter the tensor cores as float16 (also for bfloat16 queries), so scale, zero, code*scale+zero, the
+ * exact rows and q must lie within +-65504. Up to three launches: tcgen05 tiles, warp tiles, merge. */
 typedef struct vq_shared_attend_args {
     const void *q;            /* [B, H_q, S_q, D] contiguous */
     void *out;                /* [B, H_q, S_q, D] contiguous, dtype of q */
@@ -639,9 +641,9 @@ typedef struct vq_shared_attend_args {
     vq_kivi_rows prefix, own;
     void *workspace;          /* >= vq_kivi_shared_attend_workspace_bytes(args), 16-byte aligned */
     int64_t workspace_bytes;
-    int32_t variant;          /* 0 = choose; 1 = warp tiles for the prefix too; 2 = the tcgen05 kernel
-                                 for the prefix */
-    int32_t n_splits;         /* context splits of the prefix; 0 = choose */
+    int32_t variant;          /* 0 = choose by size; 1 = warp tiles for both parts; 2 = the tcgen05 kernel for
+                                 the prefix (and for own tokens with more than 32 query rows a kv head) */
+    int32_t n_splits;         /* token splits of the prefix (at most 64; tcgen05: 32); 0 = choose */
 } vq_shared_attend_args;
 int64_t vq_kivi_shared_attend_workspace_bytes(const vq_shared_attend_args *args);
 /* vq_kivi_attend_status also reports the bounded waits of this call's kernels. */

@@ -411,3 +411,19 @@ def test_a_nan_that_is_seen_stays_in_its_rows():
         bad[3, 1] = False
         bad[9, :, :, 5] = False
         assert not bool(bad.any())
+
+
+def test_a_wait_that_runs_out_is_reported_once():
+    """The bounded waits' error path: a barrier that nothing arms, waited for behind the work (which stays right)."""
+    from veloxquant_mlx_b200 import VQLibraryError
+
+    q = torch.randn(40, 2, 1, 128, device=DEV, generator=_gen(80)).half()
+    pre = make_store(1, 1, 128, 4, 512, 9, HF, 81)
+    want = kivi_shared_prefix_attend(q, pre[0], None, 0.1, variant=2)
+    kernels.attend_status()
+    assert kernels.tune("shared_wait_test", 1) == 0
+    out = kivi_shared_prefix_attend(q, pre[0], None, 0.1, variant=2)
+    with pytest.raises(VQLibraryError, match="TIMEOUT.*shared"):
+        kernels.attend_status()
+    kernels.attend_status()
+    assert torch.equal(out, want) and kernels.tune("shared_wait_test", 0) == 0

@@ -70,7 +70,7 @@ VQ_ATTEND_OVERLAP_PREVIOUS = 1
 VQ_ATTEND_CAUSAL = 2
 VQ_MAX_PEERS = 16
 (VQ_KNOB_ATTEND_STAGES, VQ_KNOB_ATTEND_WAVES, VQ_KNOB_VQ_SEARCH, VQ_KNOB_ATTEND_WAIT_TEST,
- VQ_KNOB_VQ_WAIT_TEST) = range(5)
+ VQ_KNOB_VQ_WAIT_TEST, VQ_KNOB_SHARED_WAIT_TEST) = range(6)
 
 
 class KiviSinks(C.Structure):

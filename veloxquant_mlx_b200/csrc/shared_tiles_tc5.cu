@@ -20,8 +20,12 @@
 // the row's own thread. That S of step i + 1 is complete implies that P V of step i is (MMAs of one
 // thread complete in order), so no further wait is needed.
 //
-// Budget of a token tile with two row tiles at 4 bits, in SM clocks: MMAs 2048, exponentials 2048 (16 a
-// clock), instruction issue about 2400, HBM 1040.
+// Measured at 4 bits in bfloat16: 256 query rows of each of 8 kv heads behind 32K tokens, 50 us; 8192 rows
+// behind 8K tokens, 340 us = 0.81 PFLOP/s, 49 % of the measured bfloat16 rate. A pair of row tiles takes
+// about 4300 clocks a token tile, against 2048 for the MMAs, 2048 for the exponentials (16 a clock), 1000 for
+// HBM and about 2400 of instruction issue: what bounds it is the chain of one stream (scores 700, their
+// shared-memory operands being as long as the MMAs; weights 2600 to 3000 beside the other stream's and the
+// decoding warps; the last half of the output 240; hand-overs 600), of which two run side by side.
 //
 // Every wait is bounded; a role that gives up raises a flag (reported by vq_kivi_attend_status), leaves its
 // loop, and the CTA still waits (bounded) for its MMAs and frees its tensor memory.
@@ -44,8 +48,8 @@ __device__ int g_shared_timeout = 0;
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-    for (uint32_t i = 0; i < kSpin; ++i) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t limit = kSpin) {
+    for (uint32_t i = 0; i < limit; ++i) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -173,6 +177,7 @@ struct TileParams {
     const int32_t *own_start;
     float scale_log2;
     int H_q, H_kv, S_q, G, causal;
+    int wait_test;    // self-test: also wait (briefly, behind all the work) on a barrier that nothing arms
     SharedPartials parts;
     Part prefix, own;
 };
@@ -203,7 +208,7 @@ struct Layout {
     __device__ static __forceinline__ uint32_t at(int r, int c) { return (uint32_t)((c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 };
 
-enum { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPReady = 10, kPVHalf = 14, kODone = 16, kDrain = 18, kBars = 19 };
+enum { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPReady = 10, kPVHalf = 14, kODone = 16, kDrain = 18, kIdle = 19, kBars = 20 };
 
 __device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
 
@@ -671,6 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
             mbar_wait(bar(kDrain), 0);
         }
     }
+    if (p.wait_test && tid == 0 && !mbar_wait(bar(kIdle), 0, 1u << 10)) gave_up = true;
     if (gave_up) atomicExch(&g_shared_timeout, 1);
     fence_before();
     __syncthreads();
@@ -730,6 +736,7 @@ int32_t shared_tiles_tc5_launch(const vq_shared_attend_args &a, const SharedPart
     p.H_q = a.H_q; p.H_kv = a.H_kv; p.S_q = a.S_q; p.G = a.H_q / a.H_kv;
     p.causal = (a.flags & VQ_ATTEND_CAUSAL) != 0;
     p.parts = parts;
+    p.wait_test = knob_take(VQ_KNOB_SHARED_WAIT_TEST);
     int64_t blocks = 0;
     auto part = [&](Part &t, const vq_kivi_rows &st, int64_t units, int64_t rows, int splits, int record0) {
         t.st = st;
