@@ -476,7 +476,9 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
         *reinterpret_cast<float4 *>(p.parts.o + rec * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         if (d == 0) *reinterpret_cast<float2 *>(p.parts.ml + rec * 2) = make_float2(mm, ll);
     }
-    wait_for_previous();  // the merge waits for this kernel alone: it must not end before the tcgen05 kernel does
+    // The merge waits for this kernel alone: it must not end before the tcgen05 kernel does. (One block waits: the
+    // others make room.)
+    if (blockIdx.x == gridDim.x - 1) wait_for_previous();
 }
 
 template <int D, int SB, typename T, int NT>
@@ -587,12 +589,10 @@ int32_t plan_of(const vq_shared_attend_args &a, const DeviceInfo &di, Plan *out)
     };
     const bool can = a.scale >= 0.f;
     VQ_REQUIRE(a.variant != 2 || (can && ip), VQ_ERR_SHAPE, "vq_kivi_shared_attend: the tcgen05 kernel needs a prefix and a scale that is not negative");
-    if (can && ip && (a.variant == 2 || (a.variant == 0 && pays(a.H_kv, all, pre))))
-        pl.prefix_tc5 = shared_tiles_tc5_splits(pre, a.H_kv, all, a.D, a.n_splits, di);
     const int64_t units = (int64_t)a.B * a.H_kv;
-    if (can && io && (a.variant == 2 ? per_req > 32 : a.variant == 0 && pays(units, per_req, own)))
-        pl.own_tc5 = shared_tiles_tc5_splits(own, units, per_req, a.D, 0, di);
-    pl.row_tile = (pl.prefix_tc5 ? per_req : all) > 8 ? 16 : 8;
+    const bool prefix_tc5 = can && ip && (a.variant == 2 || (a.variant == 0 && pays(a.H_kv, all, pre)));
+    const bool own_tc5 = can && io && (a.variant == 2 ? per_req > 32 : a.variant == 0 && pays(units, per_req, own));
+    pl.row_tile = (prefix_tc5 ? per_req : all) > 8 ? 16 : 8;
     pl.prefix_tiles = (int)ceil_div(all, pl.row_tile);
     pl.own_tiles = (int)ceil_div(per_req, pl.row_tile);
     auto splits = [&](int64_t tiles, int items) {
@@ -600,10 +600,17 @@ int32_t plan_of(const vq_shared_attend_args &a, const DeviceInfo &di, Plan *out)
         // 1 split 25 us, 2 28 us, 4 33 us)
         return (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)di.sm_count * 4 / tiles, ceil_div(items, 2 * kWarps), 64}));
     };
-    if (pl.prefix_tc5) pl.np = shared_tiles_tc5_records(all, pl.prefix_tc5);
-    else if (ip) pl.np = a.n_splits > 0 ? std::min({a.n_splits, ip, 64}) : splits((int64_t)a.H_kv * pl.prefix_tiles, ip);
-    if (pl.own_tc5) pl.no = shared_tiles_tc5_records(per_req, pl.own_tc5);
-    else if (io) pl.no = splits(units * pl.own_tiles, io);
+    if (io && !own_tc5) pl.no = splits(units * pl.own_tiles, io);
+    if (ip && !prefix_tc5) pl.np = a.n_splits > 0 ? std::min({a.n_splits, ip, 64}) : splits((int64_t)a.H_kv * pl.prefix_tiles, ip);
+    if (prefix_tc5 || own_tc5) {
+        // An SM full of warp tiles does an item a warp in 0.46 us for each block; to start and end takes 4.5 items.
+        double beside = 0.0;
+        if (io && !own_tc5)
+            beside = 0.46 * (pl.row_tile == 16 ? 1.3 : 1.0) * (a.D == 128 ? 1.0 : 0.75) * (double)(units * pl.own_tiles * pl.no) * ((double)ceil_div(io, pl.no * kWarps) + 4.5);
+        shared_tiles_tc5_splits({prefix_tc5 ? &pre : nullptr, a.H_kv, all}, {own_tc5 ? &own : nullptr, units, per_req}, a.D, a.n_splits, beside, di, &pl.prefix_tc5, &pl.own_tc5);
+        if (prefix_tc5) pl.np = pl.prefix_tc5;
+        if (own_tc5) pl.no = pl.own_tc5;
+    }
     *out = pl;
     return VQ_OK;
 }

@@ -14,12 +14,16 @@ struct SharedPartials {
     int n_splits;  // prefix splits, then own splits
 };
 
-// The tcgen05 kernel (shared_tiles_tc5.cu): the splits it uses for a store against `units` x `rows` query
-// rows; its launch for the prefix (prefix_splits > 0, records from 0) and the own tokens (own_splits > 0,
-// records from own_record0); its "a bounded wait gave up" flag. A part of at most 128 rows a unit leaves two
-// records per split.
-int shared_tiles_tc5_splits(const vq_kivi_rows &st, int64_t units, int64_t rows, int D, int wanted, const DeviceInfo &di);
-inline int shared_tiles_tc5_records(int64_t rows, int splits) { return rows > 128 ? splits : 2 * splits; }
+// The tcgen05 kernel (shared_tiles_tc5.cu): the splits it uses for the parts it takes, each `units` x `rows`
+// query rows against a store (st NULL: not that part; `wanted` > 0: so many for the prefix; `beside`: what else
+// there is to do meanwhile, in SM microseconds); its launch for the prefix (prefix_splits > 0, records from 0)
+// and the own tokens (own_splits > 0, records from own_record0), one record a split; its "a bounded wait gave
+// up" flag.
+struct Tc5Part {
+    const vq_kivi_rows *st;
+    int64_t units, rows;
+};
+void shared_tiles_tc5_splits(const Tc5Part &prefix, const Tc5Part &own, int D, int wanted, double beside, const DeviceInfo &di, int *prefix_splits, int *own_splits);
 int32_t shared_tiles_tc5_launch(const vq_shared_attend_args &a, const SharedPartials &parts, int prefix_splits, int own_splits, int own_record0,
                                 cudaStream_t stream);
 int32_t shared_tiles_tc5_take_timeout(int *flag);

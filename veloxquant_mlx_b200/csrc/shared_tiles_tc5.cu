@@ -7,7 +7,7 @@
 // memory). Each CTA keeps two such streams in flight so that the softmax of one runs under the MMAs
 // of the other:
 //   more than 128 rows: two row tiles share every decoded token tile;
-//   up to 128 rows:     one row tile, the streams take token tiles in turn and leave two partial records.
+//   up to 128 rows:     one row tile, the streams take token tiles in turn and are joined at the end.
 // Roles: warps 0-3 and 4-7 the softmax of stream 0 and 1 (a thread owns a row: no exchange between
 // lanes), warps 8-11 decode keys, 12-15 values, warp 16 issues the MMAs. Codes go from global memory to
 // registers one tile ahead (a register is refilled as soon as its code is used), through one fused
@@ -201,7 +201,9 @@ struct Layout {
     static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE;   // two Q tiles, two stages of K and V
     static constexpr int OUT_ROW = 4 * D + 16;                // a row of O on its way out: padded, conflict-free
     static constexpr int OUT = 2 * kTile * OUT_ROW;           // (over the tiles, when they are done with)
-    static constexpr int BARS = 6 * TILE > OUT ? 6 * TILE : OUT;
+    static constexpr int ML = OUT;                            // (m, l) of every thread's row
+    static constexpr int BARS = 6 * TILE;
+    static_assert(OUT + 2 * kTile * 8 <= BARS, "rows on their way out fit over the tiles");
     // padded past half an SM's shared memory: one CTA an SM, as it takes all of tensor memory
     static constexpr int BYTES = BARS + 256 > 120 * 1024 ? BARS + 256 : 120 * 1024;
     // 16-byte chunk `c` (0 .. D/8) of row `r`
@@ -410,13 +412,17 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
         if (n_steps > 1) wait(kODone + 1, 0);
         fence_after();
         const bool live = r < n_rows;
-        const int64_t rec = live ? out_row(r) * p.parts.n_splits + part.record0 + (two ? split : 2 * split + s) : 0;
+        const int64_t rec = live ? out_row(r) * p.parts.n_splits + part.record0 + split : 0;
         uint8_t *rows = smem + warp * 32 * L::OUT_ROW, *mine = rows + lane * L::OUT_ROW;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
             float v[32];
             tmem_ld32(to + c, v);
             tmem_ld_wait(v);
+            if (n_mine == 0) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) v[k] = 0.f;
+            }
             // (channels i and i + 4 of a spread chunk are columns 2 i and 2 i + 1)
             float4 *at = reinterpret_cast<float4 *>(mine + 4 * c);
 #pragma unroll
@@ -425,16 +431,36 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
                 at[k / 4 + 1] = HALF ? make_float4(v[k + 1], v[k + 3], v[k + 5], v[k + 7]) : make_float4(v[k + 4], v[k + 5], v[k + 6], v[k + 7]);
             }
         }
-        if (live) *reinterpret_cast<float2 *>(p.parts.ml + rec * 2) = make_float2(m, l);
-        __syncwarp();
         constexpr int LPR = D / 4;  // lanes that write a row
+        if (two) {
+            if (live) *reinterpret_cast<float2 *>(p.parts.ml + rec * 2) = make_float2(m, l);
+            __syncwarp();
 #pragma unroll 4
-        for (int i = 0; i < 32; i += 32 / LPR) {
-            const int from = i + lane / LPR;
-            const float4 v = *reinterpret_cast<const float4 *>(rows + from * L::OUT_ROW + 16 * (lane % LPR));
-            const int64_t to_rec = __shfl_sync(0xffffffffu, rec, from);
-            if (row0 + (two ? s * kTile : 0) + (warp & 3) * 32 + from < n_rows)
-                *reinterpret_cast<float4 *>(p.parts.o + to_rec * D + 4 * (lane % LPR)) = n_mine > 0 ? v : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < 32; i += 32 / LPR) {
+                const int from = i + lane / LPR;
+                const float4 v = *reinterpret_cast<const float4 *>(rows + from * L::OUT_ROW + 16 * (lane % LPR));
+                const int64_t to_rec = __shfl_sync(0xffffffffu, rec, from);
+                if (r - lane + from < n_rows) *reinterpret_cast<float4 *>(p.parts.o + to_rec * D + 4 * (lane % LPR)) = v;
+            }
+        } else {  // the streams' two records of a row become one; each stream's warps write half of the rows
+            float2 *ml = reinterpret_cast<float2 *>(smem + L::ML) + (warp & 3) * 32 + lane;
+            ml[s * kTile] = make_float2(m, l);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float2 a = ml[0], b = ml[kTile];
+            const float mm = fmaxf(a.x, b.x), base = mm == -INFINITY ? 0.f : mm, fa = ex2(a.x - base), fb = ex2(b.x - base);
+            if (live && s == 0) *reinterpret_cast<float2 *>(p.parts.ml + rec * 2) = make_float2(mm, a.y * fa + b.y * fb);
+            rows = smem + (warp & 3) * 32 * L::OUT_ROW;
+#pragma unroll 4
+            for (int i = 16 * s; i < 16 * s + 16; i += 32 / LPR) {
+                const int from = i + lane / LPR;
+                const uint8_t *at = rows + from * L::OUT_ROW + 16 * (lane % LPR);
+                const float4 x = *reinterpret_cast<const float4 *>(at), y = *reinterpret_cast<const float4 *>(at + kTile * L::OUT_ROW);
+                const float f = __shfl_sync(0xffffffffu, fa, from), g = __shfl_sync(0xffffffffu, fb, from);
+                const int64_t to_rec = __shfl_sync(0xffffffffu, rec, from);
+                if (r - lane + from < n_rows)
+                    *reinterpret_cast<float4 *>(p.parts.o + to_rec * D + 4 * (lane % LPR)) =
+                        make_float4(x.x * f + y.x * g, x.y * f + y.y * g, x.z * f + y.z * g, x.w * f + y.w * g);
+            }
         }
     } else if (warp < 12) {
         fewer_registers<HALF>();
@@ -689,6 +715,16 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
 int tiles_of(const vq_kivi_rows &st) { return (int)(ceil_div(st.n_quant, kTile) + ceil_div(st.n_res, kTile)); }
 int row_blocks_of(int64_t rows) { return (int)ceil_div(rows, rows > kTile ? 2 * kTile : kTile); }
 
+// When `n1` CTAs of `d1` microseconds and then `n2` of `d2`, one an SM, are done
+double done_after(int64_t n1, double d1, int64_t n2, double d2, int sms) {
+    const int64_t rest = n1 % sms;                 // SMs that are busy d1 longer than the others
+    const double t0 = (double)(n1 / sms) * d1, t1 = rest ? t0 + d1 : t0;
+    if (n2 == 0) return t1;
+    const double late = d1 / d2;
+    for (int64_t k = std::max<int64_t>(1, (int64_t)std::min((double)n2 / (double)(sms - rest), ((double)n2 + (double)rest * late) / sms));; ++k)
+        if ((sms - rest) * k + rest * std::max<int64_t>(0, (int64_t)((double)k - late)) >= n2) return std::max(t1, t0 + (double)k * d2);
+}
+
 template <int D, int SB, typename T>
 int32_t launch(const TileParams &p, unsigned blocks, cudaStream_t st) {
     static std::atomic<uint64_t> allowed{0};
@@ -707,23 +743,37 @@ int32_t launch_bits(int sb, const TileParams &p, unsigned blocks, cudaStream_t s
 
 }  // namespace
 
-// Splits of one part along its tokens: the count with the smallest estimate in microseconds. A wave of CTAs
-// (one an SM) takes 8 for setup and epilogue and 2.5 (head_dim 64: 2) a token tile with two row tiles, or a
-// pair of token tiles with one; a partial record of a row costs 0.2 ns more (written here, read by the
-// merge). Measured at 16 requests behind 8K tokens: 6 splits 26.8, 10 22.3, 18 23.4; 96 requests behind 4K,
-// head_dim 64: 6 23.1, 11 19.6, 18 22.4; 64 requests behind 32K: 12 84.2, 18 71.8.
-int shared_tiles_tc5_splits(const vq_kivi_rows &st, int64_t units, int64_t rows, int D, int wanted, const DeviceInfo &di) {
-    const int tiles = tiles_of(st), most = std::min(tiles, 32);
-    if (wanted > 0) return std::min(wanted, most);
-    const int64_t ctas = units * row_blocks_of(rows);
-    int best = 1;
+// Splits of the parts along their tokens: the counts with the smallest estimate in microseconds. A CTA (one an
+// SM) takes 15 in all but its token tiles, 2.6 a tile with two row tiles and 2.25 with one. The SMs that the
+// prefix leaves idle do `beside`, the own tokens' warp tiles, in SM microseconds, from 5 after its start; what
+// is left of that comes behind, on all SMs. A partial record of a row costs 0.04 ns more (written here, read
+// by the merge). Fitted to 95 calls of 32 to 8192 query rows behind 1K to 32K tokens, each measured at every
+// split count of the prefix: the count chosen is 1.6 % slower than the best one in the mean, 13 % at worst.
+void shared_tiles_tc5_splits(const Tc5Part &prefix, const Tc5Part &own, int D, int wanted, double beside, const DeviceInfo &di, int *prefix_splits, int *own_splits) {
+    struct Side {
+        int tiles, most;
+        int64_t ctas, rows;
+        double step;
+        Side(const Tc5Part &p, int D, int limit)
+            : tiles(p.st ? tiles_of(*p.st) : 0), most(std::min(tiles, limit)), ctas(p.st ? p.units * row_blocks_of(p.rows) : 0), rows(p.units * p.rows),
+              step((p.rows > kTile ? 2.6 : 2.25) * (D == 128 ? 1.0 : 0.9)) {}
+        double time(int s) const { return s ? 15.0 + step * (double)ceil_div(tiles, s) : 0.0; }
+    };
+    const Side a(prefix, D, 32), b(own, D, 8);
+    const int a_lo = !a.tiles ? 0 : wanted > 0 ? std::min(wanted, a.most) : 1, a_hi = wanted > 0 ? a_lo : a.most;
     double least = 1e30;
-    for (int s = 1; s <= most; ++s) {
-        const int64_t longest = ceil_div(tiles, s), steps = rows > kTile ? longest : ceil_div(longest, 2);
-        const double us = (double)ceil_div(ctas * s, di.sm_count) * (8.0 + (D == 128 ? 2.5 : 2.0) * (double)steps) + 2e-4 * 2 * kTile * (double)(ctas * s);
-        if (us < least) { least = us; best = s; }
+    for (int t = b.tiles ? 1 : 0; t <= b.most; ++t) {
+        const double bt = b.time(t);
+        for (int s = a_lo; s <= a_hi; ++s) {
+            const double at = a.time(s);
+            double us = done_after(a.ctas * s, at, b.ctas * t, bt, di.sm_count) + 4e-5 * (double)(a.rows * s + b.rows * t) * D / 128;
+            if (beside > 0.0) {
+                const double idle = (double)(ceil_div(a.ctas * s, di.sm_count) * di.sm_count - a.ctas * s) * (at - 5.0);
+                if (beside > idle) us += 1.4 + (beside - idle) / di.sm_count;
+            }
+            if (us < least) { least = us; *prefix_splits = s; *own_splits = t; }
+        }
     }
-    return best;
 }
 
 int32_t shared_tiles_tc5_launch(const vq_shared_attend_args &a, const SharedPartials &parts, int prefix_splits, int own_splits, int own_record0,
