@@ -596,9 +596,11 @@ int32_t plan_of(const vq_shared_attend_args &a, const DeviceInfo &di, Plan *out)
     pl.prefix_tiles = (int)ceil_div(all, pl.row_tile);
     pl.own_tiles = (int)ceil_div(per_req, pl.row_tile);
     auto splits = [&](int64_t tiles, int items) {
-        // as many CTAs as fit the GPU at once, but at least two work items a warp (512 units of 26 items:
-        // 1 split 25 us, 2 28 us, 4 33 us)
-        return (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)di.sm_count * 4 / tiles, ceil_div(items, 2 * kWarps), 64}));
+        // As many CTAs as fit the GPU at once, but at least two work items a warp (512 units of 26 items: 1 split
+        // 25 us, 2 28 us, 4 33 us), or one while every CTA has an SM to itself (8 units of 14 items: 2 splits 8.3 us, 4
+        // 6.9, 8 6.9, 16 7.5; of 32: 4 splits 6.6, 8 5.6, 16 5.8).
+        const int64_t few = ceil_div(items, 2 * kWarps), more = std::min(ceil_div(items, kWarps), (int64_t)di.sm_count / tiles);
+        return (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)di.sm_count * 4 / tiles, std::max<int64_t>(few, more), 64}));
     };
     if (io && !own_tc5) pl.no = splits(units * pl.own_tiles, io);
     if (ip && !prefix_tc5) pl.np = a.n_splits > 0 ? std::min({a.n_splits, ip, 64}) : splits((int64_t)a.H_kv * pl.prefix_tiles, ip);
