@@ -605,10 +605,10 @@ int32_t plan_of(const vq_shared_attend_args &a, const DeviceInfo &di, Plan *out)
     if (io && !own_tc5) pl.no = splits(units * pl.own_tiles, io);
     if (ip && !prefix_tc5) pl.np = a.n_splits > 0 ? std::min({a.n_splits, ip, 64}) : splits((int64_t)a.H_kv * pl.prefix_tiles, ip);
     if (prefix_tc5 || own_tc5) {
-        // An SM full of warp tiles does an item a warp in 0.46 us for each block; to start and end takes 4.5 items.
+        // An SM full of warp tiles does an item a warp in 0.5 us for each block; to start and end takes three items.
         double beside = 0.0;
         if (io && !own_tc5)
-            beside = 0.46 * (pl.row_tile == 16 ? 1.3 : 1.0) * (a.D == 128 ? 1.0 : 0.75) * (double)(units * pl.own_tiles * pl.no) * ((double)ceil_div(io, pl.no * kWarps) + 4.5);
+            beside = 0.5 * (pl.row_tile == 16 ? 1.2 : 1.0) * (a.D == 128 ? 1.0 : 0.85) * (double)(units * pl.own_tiles * pl.no) * ((double)ceil_div(io, pl.no * kWarps) + 3.0);
         shared_tiles_tc5_splits({prefix_tc5 ? &pre : nullptr, a.H_kv, all}, {own_tc5 ? &own : nullptr, units, per_req}, a.D, a.n_splits, beside, di, &pl.prefix_tc5, &pl.own_tc5);
         if (prefix_tc5) pl.np = pl.prefix_tc5;
         if (own_tc5) pl.no = pl.own_tc5;

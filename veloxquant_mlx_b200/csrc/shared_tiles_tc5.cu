@@ -744,20 +744,20 @@ int32_t launch_bits(int sb, const TileParams &p, unsigned blocks, cudaStream_t s
 }  // namespace
 
 // Splits of the parts along their tokens: the counts with the smallest estimate in microseconds. A CTA (one an
-// SM) takes 15 in all but its token tiles, 2.6 a tile with two row tiles and 2.25 with one. The SMs that the
-// prefix leaves idle do `beside`, the own tokens' warp tiles, in SM microseconds, from 5 after its start; what
-// is left of that comes behind, on all SMs. A partial record of a row costs 0.04 ns more (written here, read
-// by the merge). Fitted to 95 calls of 32 to 8192 query rows behind 1K to 32K tokens, each measured at every
-// split count of the prefix: the count chosen is 1.6 % slower than the best one in the mean, 13 % at worst.
+// SM) takes 3.0 a token tile and 13 for the rest with two row tiles, 3.2 and 16 with one. The SMs that the
+// prefix leaves idle do `beside`, the own tokens' warp tiles, in SM microseconds, from 3 after its start; what
+// is left of that comes behind, on all SMs. A partial record of a row costs 0.2 ns more (written here, read
+// by the merge). Fitted to 105 calls of 32 to 8192 query rows behind 1K to 32K tokens that come from HBM, each
+// measured at every split count of the prefix: the count chosen is 1.6 % slower than the best one in the mean.
 void shared_tiles_tc5_splits(const Tc5Part &prefix, const Tc5Part &own, int D, int wanted, double beside, const DeviceInfo &di, int *prefix_splits, int *own_splits) {
     struct Side {
         int tiles, most;
         int64_t ctas, rows;
-        double step;
+        double rest, step;
         Side(const Tc5Part &p, int D, int limit)
             : tiles(p.st ? tiles_of(*p.st) : 0), most(std::min(tiles, limit)), ctas(p.st ? p.units * row_blocks_of(p.rows) : 0), rows(p.units * p.rows),
-              step((p.rows > kTile ? 2.6 : 2.25) * (D == 128 ? 1.0 : 0.9)) {}
-        double time(int s) const { return s ? 15.0 + step * (double)ceil_div(tiles, s) : 0.0; }
+              rest(p.rows > kTile ? 13.0 : 16.0), step((p.rows > kTile ? 3.0 : 3.2) * (D == 128 ? 1.0 : 0.8)) {}
+        double time(int s) const { return s ? rest + step * (double)ceil_div(tiles, s) : 0.0; }
     };
     const Side a(prefix, D, 32), b(own, D, 8);
     const int a_lo = !a.tiles ? 0 : wanted > 0 ? std::min(wanted, a.most) : 1, a_hi = wanted > 0 ? a_lo : a.most;
@@ -766,9 +766,9 @@ void shared_tiles_tc5_splits(const Tc5Part &prefix, const Tc5Part &own, int D, i
         const double bt = b.time(t);
         for (int s = a_lo; s <= a_hi; ++s) {
             const double at = a.time(s);
-            double us = done_after(a.ctas * s, at, b.ctas * t, bt, di.sm_count) + 4e-5 * (double)(a.rows * s + b.rows * t) * D / 128;
+            double us = done_after(a.ctas * s, at, b.ctas * t, bt, di.sm_count) + 2e-4 * (double)(a.rows * s + b.rows * t) * D / 128;
             if (beside > 0.0) {
-                const double idle = (double)(ceil_div(a.ctas * s, di.sm_count) * di.sm_count - a.ctas * s) * (at - 5.0);
+                const double idle = (double)(ceil_div(a.ctas * s, di.sm_count) * di.sm_count - a.ctas * s) * (at - 3.0);
                 if (beside > idle) us += 1.4 + (beside - idle) / di.sm_count;
             }
             if (us < least) { least = us; *prefix_splits = s; *own_splits = t; }
