@@ -643,7 +643,7 @@ typedef struct vq_shared_attend_args {
     int64_t workspace_bytes;
     int32_t variant;          /* 0 = choose by size; 1 = warp tiles for both parts; 2 = the tcgen05 kernel for
                                  the prefix (and for own tokens with more than 32 query rows a kv head) */
-    int32_t n_splits;         /* token splits of the prefix (at most 64; tcgen05: 32); 0 = choose */
+    int32_t n_splits;         /* token splits of the prefix (at most 64); 0 = choose */
 } vq_shared_attend_args;
 int64_t vq_kivi_shared_attend_workspace_bytes(const vq_shared_attend_args *args);
 /* vq_kivi_attend_status also reports the bounded waits of this call's kernels. */

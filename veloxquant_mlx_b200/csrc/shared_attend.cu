@@ -581,11 +581,11 @@ int32_t plan_of(const vq_shared_attend_args &a, const DeviceInfo &di, Plan *out)
     const int ip = pre.n_quant / kGroup + (int)ceil_div(pre.n_res, kExact), io = own.n_quant / kGroup + (int)ceil_div(own.n_res, kExact);
     // The tcgen05 kernel decodes a token once for 128 or 256 query rows, the warp tiles for 8 or 16, but it
     // takes 5 us longer to start and end. Measured with 8 kv heads, warp tiles / tcgen05 in us: 64 rows
-    // behind 1K tokens 10.4 / 12.6, 2K 14.1 / 13.3, 8K 29 / 19; 32 rows behind 2K 9.7 / 12.7, 8K 19.9 / 18.3;
-    // 16 rows behind 32K 27.6 / 32.2; own tokens, 1 request of 128 rows over 662: 14.6 / 18.5, of 256: 21.8 /
-    // 17.2; 8 of 36 over 100: 14.3 / 15.4, over 662: 26.6 / 23.0. It takes scales that are not negative.
+    // behind 1K tokens 10.3 / 12.2, 2K 13.9 / 12.8, 8K 28.7 / 16.7; 256 behind 512: 18.6 / 15.6; 32 behind 2K
+    // 9.6 / 12.4, 4K 11.8 / 13.4, 8K 19.6 / 16.1; 16 behind 32K 27.1 / 30.3; own tokens, 1 request of 256 rows
+    // over 662: 22.5 / 16.7; 8 of 36 over 662: 26.5 / 19.9. It takes scales that are not negative.
     auto pays = [&](int64_t units, int64_t rows, const vq_kivi_rows &st) {
-        return rows >= 32 && (double)units * (double)rows * ((double)st.n_quant + st.n_res) >= 1 << 20;
+        return rows >= 32 && (double)units * (double)rows * ((double)st.n_quant + st.n_res) >= (rows < 64 && units < 32 ? 2 << 20 : 1 << 20);
     };
     const bool can = a.scale >= 0.f;
     VQ_REQUIRE(a.variant != 2 || (can && ip), VQ_ERR_SHAPE, "vq_kivi_shared_attend: the tcgen05 kernel needs a prefix and a scale that is not negative");

@@ -751,18 +751,20 @@ int32_t launch_bits(int sb, const TileParams &p, unsigned blocks, cudaStream_t s
 // measured at every split count of the prefix: the count chosen is 1.6 % slower than the best one in the mean.
 void shared_tiles_tc5_splits(const Tc5Part &prefix, const Tc5Part &own, int D, int wanted, double beside, const DeviceInfo &di, int *prefix_splits, int *own_splits) {
     struct Side {
-        int tiles, most;
+        int tiles;
         int64_t ctas, rows;
         double rest, step;
-        Side(const Tc5Part &p, int D, int limit)
-            : tiles(p.st ? tiles_of(*p.st) : 0), most(std::min(tiles, limit)), ctas(p.st ? p.units * row_blocks_of(p.rows) : 0), rows(p.units * p.rows),
-              rest(p.rows > kTile ? 13.0 : 16.0), step((p.rows > kTile ? 3.0 : 3.2) * (D == 128 ? 1.0 : 0.8)) {}
+        int most;  // two waves, or four splits
+        Side(const Tc5Part &p, int D, int sms)
+            : tiles(p.st ? tiles_of(*p.st) : 0), ctas(p.st ? p.units * row_blocks_of(p.rows) : 0), rows(p.units * p.rows),
+              rest(p.rows > kTile ? 13.0 : 16.0), step((p.rows > kTile ? 3.0 : 3.2) * (D == 128 ? 1.0 : 0.8)),
+              most(ctas ? (int)std::min<int64_t>({(int64_t)tiles, 64, std::max<int64_t>(4, 2 * sms / ctas)}) : 0) {}
         double time(int s) const { return s ? rest + step * (double)ceil_div(tiles, s) : 0.0; }
     };
-    const Side a(prefix, D, 32), b(own, D, 8);
-    const int a_lo = !a.tiles ? 0 : wanted > 0 ? std::min(wanted, a.most) : 1, a_hi = wanted > 0 ? a_lo : a.most;
+    const Side a(prefix, D, di.sm_count), b(own, D, di.sm_count);
+    const int a_lo = !a.tiles ? 0 : wanted > 0 ? std::min({wanted, a.tiles, 64}) : 1, a_hi = wanted > 0 ? a_lo : a.most;
     double least = 1e30;
-    for (int t = b.tiles ? 1 : 0; t <= b.most; ++t) {
+    for (int t = b.tiles ? 1 : 0; t <= std::min(b.most, 8); ++t) {
         const double bt = b.time(t);
         for (int s = a_lo; s <= a_hi; ++s) {
             const double at = a.time(s);
