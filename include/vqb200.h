@@ -614,7 +614,7 @@ typedef struct vq_kivi_rows {
     const float *v_scale, *v_zero;              /* rows [token][D/group] */
     const void *k_res, *v_res;                  /* rows [token][D] in q's dtype, 16-byte aligned */
     int64_t k_codes_stride_bh, v_codes_stride_bh; /* bytes between (batch, kv head) slabs */
-    int64_t k_param_stride_bh, v_param_stride_bh; /* floats */
+    int64_t k_param_stride_bh, v_param_stride_bh; /* floats, multiples of 4 */
     int64_t res_stride_bh;                      /* elements */
     int32_t n_quant;                            /* packed tokens, a multiple of group */
     int32_t n_res;                              /* exact rows */

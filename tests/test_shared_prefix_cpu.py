@@ -112,3 +112,21 @@ def test_struct_sizes_match_header(tmp_path):
     assert (r.factor, r.pos_stride_b, r.pos_stride_s, r.pos_offset, r.turns) == (37.0, 38, 39, 40, 41)
     k = _lib.KiviRowsArgs.from_buffer_copy(_lib.KIVI_ROWS_PACK.pack(*range(1, 16)))
     assert (k.k_codes, k.v_res, k.k_codes_stride_bh, k.res_stride_bh, k.n_quant, k.n_res) == (1, 8, 9, 13, 14, 15)
+
+
+def test_value_scales_whose_slabs_would_be_off_16_bytes_are_refused():
+    """head_dim 64 has two scales a token: with an odd number of tokens the next head's would start 8 bytes off."""
+    from veloxquant_mlx_b200 import _lib
+
+    odd = dict(v_scale=torch.zeros(1, 2, 65, 2), v_zero=torch.zeros(1, 2, 65, 2))
+    with pytest.raises(ValueError, match="even number of tokens"):
+        KiviRows(**{**_store(D=64), **odd})
+    good = KiviRows(**_store(D=64))._args
+    head = _lib.SHARED_ATTEND_HEAD.pack(64, 64, 0, 0, 0, 1, 2, 2, 1, 64, 4, 32, 0.1, 0)
+    tail = _lib.SHARED_ATTEND_TAIL.pack(0, 0, 0, 0)
+    need = _lib.lib().vq_kivi_shared_attend_workspace_bytes
+    assert need(head + good + bytes(_lib.KIVI_ROWS_PACK.size) + tail) > 0
+    fields = list(_lib.KIVI_ROWS_PACK.unpack(good))
+    assert fields[11] == 128  # v_param_stride_bh
+    fields[11] = 130
+    assert need(head + _lib.KIVI_ROWS_PACK.pack(*fields) + bytes(_lib.KIVI_ROWS_PACK.size) + tail) == 0

@@ -427,3 +427,19 @@ def test_a_wait_that_runs_out_is_reported_once():
         kernels.attend_status()
     kernels.attend_status()
     assert torch.equal(out, want) and kernels.tune("shared_wait_test", 0) == 0
+
+
+@pytest.mark.parametrize("B,H,G,n_pre,n_own,Sq", [(3, 8, 8, 96, 5, 4), (40, 2, 2, 4096, 1, 1), (9, 1, 16, 20000, 40, 1), (2, 4, 4, 300, 290, 40)])
+def test_parts_that_end_in_either_order(B, H, G, n_pre, n_own, Sq):
+    """The own tokens' kernel runs beside the prefix's and may be done long before or long after it; one and two row
+    tiles, one token tile for two streams, own tokens on tcgen05 too. Twenty calls in a row give the same bits."""
+    pre, _ = make_store(1, H, 128, 4, n_pre // 32 * 32, n_pre % 32, BF, 90)
+    own, _ = make_store(B, H, 128, 4, n_own // 32 * 32, n_own % 32, BF, 91)
+    q = torch.randn(B, H * G, Sq, 128, device=DEV, generator=_gen(92)).to(BF)
+    first = kivi_shared_prefix_attend(q, pre, own, 0.088, variant=2)
+    warp_tiles = kivi_shared_prefix_attend(q, pre, own, 0.088, variant=1)
+    # (two roundings of the weights and of the output apart, on values of at most about 4: 4 (2 * 2^-11 + 2 * 2^-8) < 0.04)
+    assert float((first.float() - warp_tiles.float()).abs().max()) < 0.04
+    for _ in range(20):
+        assert torch.equal(kivi_shared_prefix_attend(q, pre, own, 0.088, variant=2), first)
+    kernels.attend_status()

@@ -639,7 +639,7 @@ int32_t validate(const vq_shared_attend_args &a) {
             VQ_REQUIRE(s->k_codes && s->v_codes && s->k_scale && s->k_zero && s->v_scale && s->v_zero, VQ_ERR_SHAPE, "%s: %s: a packed tensor is NULL", fn, which);
             VQ_REQUIRE(is_aligned(s->k_codes, 16) && is_aligned(s->v_codes, 16) && is_aligned(s->k_scale, 16) && is_aligned(s->k_zero, 16) &&
                            is_aligned(s->v_scale, 16) && is_aligned(s->v_zero, 16) && s->k_codes_stride_bh % 16 == 0 && s->v_codes_stride_bh % 16 == 0 &&
-                           s->k_param_stride_bh % 4 == 0,
+                           s->k_param_stride_bh % 4 == 0 && s->v_param_stride_bh % 4 == 0,
                        VQ_ERR_ALIGN, "%s: %s: packed tensors and their slabs must be 16-byte aligned", fn, which);
         }
         if (s->n_res) {
@@ -678,7 +678,7 @@ int32_t launch_all(const vq_shared_attend_args &a, const Plan &pl, const DeviceI
         if (rc != VQ_OK) return rc;
     }
     if (blocks) {
-        // (behind the tcgen05 kernel: its blocks fill the SMs as that kernel's finish)
+        // (behind the tcgen05 kernel: its blocks take the SMs that kernel leaves, then those where it is done)
         const bool wide = pl.row_tile == 16;
         const unsigned nb = (unsigned)blocks;
         int32_t rc;

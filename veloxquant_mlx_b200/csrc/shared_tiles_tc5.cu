@@ -20,7 +20,7 @@
 // the row's own thread. That S of step i + 1 is complete implies that P V of step i is (MMAs of one
 // thread complete in order), so no further wait is needed.
 //
-// Measured at 4 bits in bfloat16: 256 query rows of each of 8 kv heads behind 32K tokens, 50 us; 8192 rows
+// Measured at 4 bits in bfloat16: 256 query rows of each of 8 kv heads behind 32K tokens, 18 splits, 50 us; 8192 rows
 // behind 8K tokens, 340 us = 0.81 PFLOP/s, 49 % of the measured bfloat16 rate. A pair of row tiles takes
 // about 4300 clocks a token tile, against 2048 for the MMAs, 2048 for the exponentials (16 a clock), 1000 for
 // HBM and about 2400 of instruction issue: what bounds it is the chain of one stream (scores 700, their

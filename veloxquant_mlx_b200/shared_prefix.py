@@ -74,6 +74,8 @@ class KiviRows:
                 raise ValueError(f"{fn}: k_scale / k_zero must be equal [{B}, {H}, groups, {D}], got {tuple(k_scale.shape)} / {tuple(k_zero.shape)}")
             if v_scale.shape != v_zero.shape or v_scale.shape[3] != D // _GROUP:
                 raise ValueError(f"{fn}: v_scale / v_zero must be equal [{B}, {H}, tokens, {D // _GROUP}], got {tuple(v_scale.shape)} / {tuple(v_zero.shape)}")
+            if v_scale.shape[2] * v_scale.shape[3] % 4:
+                raise ValueError(f"{fn}: v_scale / v_zero must hold an even number of tokens at head_dim 64, got {v_scale.shape[2]}")
             cap = min(cap, k_scale.shape[2] * _GROUP, v_scale.shape[2])
             pointers = tuple(t.data_ptr() for t in (k_codes, v_codes, k_scale, k_zero, v_scale, v_zero))
             if any(packed[n].data_ptr() % 16 for n in packed):
