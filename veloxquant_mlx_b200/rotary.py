@@ -25,6 +25,9 @@ _NO_STRIDE = (0, 0, 0)
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
+_empty_like = torch.empty_like
+
+
 def _empty(x: torch.Tensor) -> torch.Tensor:
     """A contiguous tensor like ``x`` (empty_like costs a third of torch.empty, but keeps strides)."""
     return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -206,33 +209,31 @@ class RotaryEmbedding:
             raise ValueError(f"{fn}: positions are on {positions.device}, q on {device}")
         return positions, sb, st[-1], 0
 
-    def _launch(self, fn, q, q_out, k, k_out, k_out_stride, v, v_out, v_out_stride, positions, inverse) -> None:
-        """``q`` to the tensor ``q_out``; ``k`` turned and ``v`` copied to addresses (or None)."""
+    def _launch(self, fn, q, xs, q_out, k, ks, k_out, k_out_strides, v_ptr, Hv, vs, v_out, v_out_strides, positions, inverse) -> None:
+        """``q`` (strides ``xs``) to the contiguous tensor ``q_out``; ``k`` turned and ``v`` copied to addresses
+        (``k`` None and ``v_ptr`` 0: not given)."""
         B, Hq, S, D = q.shape
         dev = q.device
-        pos, psb, pss, off = self._positions(fn, positions, B, S, dev)
-        x0, x1, x2, _ = q.stride()
-        y0, y1, y2, _ = q_out.stride()
         if k is None:
-            k_ptr = Hk = k0 = k1 = k2 = 0
+            k_ptr = Hk = 0
         else:
             k_ptr, Hk = k.data_ptr(), k.shape[1]
-            k0, k1, k2, _ = k.stride()
-        if v is None:
-            v_ptr = Hv = v0 = v1 = v2 = 0
+        if positions is None or type(positions) is int:
+            pos_ptr = psb = pss = 0
+            pos_bytes, off = 8, positions or 0
         else:
-            v_ptr, Hv = v.data_ptr(), v.shape[1]
-            v0, v1, v2, _ = v.stride()
-        if pos is None:
-            pos_ptr, pos_bytes = 0, 8
-        else:
-            pos_ptr, pos_bytes = pos.data_ptr(), 8 if pos.dtype is torch.int64 else 4
+            pos, psb, pss, off = self._positions(fn, positions, B, S, dev)
+            pos_ptr, pos_bytes = (0, 8) if pos is None else (pos.data_ptr(), 8 if pos.dtype is torch.int64 else 4)
+        index = dev.index
+        turns = self._turns.get(index)
+        row = S * D
         a = ROTARY_PACK.pack(
-            q.data_ptr(), k_ptr, v_ptr, q_out.data_ptr(), k_out, v_out, x0, x1, x2, k0, k1, k2, v0, v1, v2, y0, y1, y2, *k_out_stride, *v_out_stride,
+            q.data_ptr(), k_ptr, v_ptr, q_out.data_ptr(), k_out, v_out, xs[0], xs[1], xs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Hq * row, row, D,
+            k_out_strides[0], k_out_strides[1], k_out_strides[2], v_out_strides[0], v_out_strides[1], v_out_strides[2],
             Hq, Hk, Hv, _DTYPE_CODES[q.dtype], B, S, D, self.rotary_dim, self._layout_code, 1 if inverse else 0, pos_ptr, pos_bytes,
-            self.attention_factor, psb, pss, off, self._turns_on(dev))
+            self.attention_factor, psb, pss, off, self._turns_on(dev) if turns is None else turns.data_ptr())
         native = lib()
-        if dev.index == torch.cuda.current_device():  # (the usual case, without a context manager)
+        if index == torch.cuda.current_device():  # (the usual case, without a context manager)
             status = native.vq_rotary(a, stream_ptr(dev))
         else:
             with _lib.on_device(dev):
@@ -251,17 +252,24 @@ class RotaryEmbedding:
         return out[0] if k is None else out
 
     def _rotate(self, fn, q, k, positions, inverse):
-        require_cuda(q, f"{fn}: q")
-        if q.stride(3) != 1:
+        if not q.is_cuda:
+            require_cuda(q, f"{fn}: q")
+        xs = q.stride()
+        if xs[3] != 1:
             q = q.contiguous()
-        yq = _empty(q)
+            xs = q.stride()
+        yq = _empty_like(q) if q.is_contiguous() else _empty(q)
         if k is None:
-            self._launch(fn, q, yq, None, 0, _NO_STRIDE, None, 0, _NO_STRIDE, positions, inverse)
+            self._launch(fn, q, xs, yq, None, _NO_STRIDE, 0, _NO_STRIDE, 0, 0, _NO_STRIDE, 0, _NO_STRIDE, positions, inverse)
             return yq, None
-        if k.stride(3) != 1:
+        ks = k.stride()
+        if ks[3] != 1:
             k = k.contiguous()
-        yk = _empty(k)
-        self._launch(fn, q, yq, k, yk.data_ptr(), yk.stride()[:3], None, 0, _NO_STRIDE, positions, inverse)
+            ks = k.stride()
+        yk = _empty_like(k) if k.is_contiguous() else _empty(k)
+        _, H, S, D = k.shape
+        row = S * D
+        self._launch(fn, q, xs, yq, k, ks, yk.data_ptr(), (H * row, row, D), 0, 0, _NO_STRIDE, 0, _NO_STRIDE, positions, inverse)
         return yq, yk
 
     def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_res: torch.Tensor, v_res: torch.Tensor, tok_offset: int,
@@ -297,7 +305,8 @@ class RotaryEmbedding:
         out = _empty(q)
         es = k.element_size()
         ks, vs = k_res.stride(), v_res.stride()
-        self._launch(fn, q, out, k, k_res.data_ptr() + tok_offset * ks[2] * es, ks[:3], v, v_res.data_ptr() + tok_offset * vs[2] * es, vs[:3], positions, False)
+        self._launch(fn, q, q.stride(), out, k, k.stride(), k_res.data_ptr() + tok_offset * ks[2] * es, ks, v.data_ptr(), H, v.stride(),
+                     v_res.data_ptr() + tok_offset * vs[2] * es, vs, positions, False)
         return out
 
 
