@@ -143,7 +143,7 @@ __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) 
                  "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
-// 8 columns of this lane times f: float32 outputs, or pairs of half weights
+// 8 columns of this lane times f
 __device__ __forceinline__ void scale_o(uint32_t addr, float f) {
     uint32_t r[8];
     tmem_ld8(addr, r);
@@ -151,17 +151,6 @@ __device__ __forceinline__ void scale_o(uint32_t addr, float f) {
     for (int k = 0; k < 8; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * f);
     tmem_st8(addr, r);
 }
-__device__ __forceinline__ void scale_p(uint32_t addr, float f) {
-    uint32_t r[8];
-    tmem_ld8(addr, r);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&r[k]));
-        r[k] = pack_f16(x.x * f, x.y * f);
-    }
-    tmem_st8(addr, r);
-}
-
 // One of the two parts of a call: the prefix (a unit is a kv head) or the own tokens (a kv head of a request)
 struct Part {
     vq_kivi_rows st;
@@ -347,8 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
             if (!wait(kSFull + s, i & 1)) break;
             fence_after();
             float2 sum[2] = {};
-            // 32 scores (already loaded) to weights; their largest may first raise m
-            auto chunk = [&](int c, float (&v)[32]) {
+            auto largest = [&](int c, float (&v)[32]) {  // of 32 scores, the masked ones dropped
                 if (masked) {
 #pragma unroll
                     for (int k = 0; k < 32; ++k) v[k] = c + k >= lo && c + k < hi ? v[k] : -INFINITY;
@@ -359,25 +347,10 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
                     mx = max3(mx, v[k], v[k + 1]);
                     m1 = max3(m1, v[k + 2], v[k + 3]);
                 }
-                mx = fmaxf(max3(mx, m1, v[30]), v[31]) * p.scale_log2;
-                if (__any_sync(0xffffffffu, mx > m + kLazy)) {
-                    const float mn = mx > m + kLazy ? mx : m, f = m == -INFINITY ? 0.f : mn == m ? 1.f : ex2(m - mn);
-                    m = mn;
-                    l *= f;
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) { sum[k].x *= f; sum[k].y *= f; }
-                    // (weights of the first half may have been taken by now: O holds them once that P V is done)
-                    if (c >= kTile / 2) wait(kPVHalf + s, i & 1);
-                    if (i > 0 || c >= kTile / 2) {
-                        fence_after();
-#pragma unroll 1
-                        for (int k = 0; k < D; k += 8) scale_o(to + k, f);
-                    }
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-#pragma unroll 1
-                    for (int k = c & (kTile / 2); k < c; k += 16) scale_p(ts + k / 2, f);
-                }
-                const float base = m == -INFINITY ? 0.f : -m;
+                return fmaxf(max3(mx, m1, v[30]), v[31]);
+            };
+            float base;
+            auto weights = [&](int c, const float (&v)[32]) {
                 uint32_t r[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
@@ -391,18 +364,35 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
             };
             float v[32], w[32];
             tmem_ld32(ts, v);
+            tmem_ld32(ts + 32, w);
 #pragma unroll 1
-            for (int c = 0; c < kTile; c += 64) {
+            for (int c = 0; c < kTile; c += 64) {  // half of the tokens: their largest score may first raise m
                 tmem_ld_wait(v);
-                tmem_ld32(ts + c + 32, w);
-                chunk(c, v);
                 tmem_ld_wait(w);
-                if (c + 64 < kTile) tmem_ld32(ts + c + 64, v);
-                chunk(c + 32, w);
+                const float m0 = largest(c, v), mx = fmaxf(m0, largest(c + 32, w)) * p.scale_log2;
+                if (__any_sync(0xffffffffu, mx > m + kLazy)) {
+                    const float mn = mx > m + kLazy ? mx : m, f = m == -INFINITY ? 0.f : mn == m ? 1.f : ex2(m - mn);
+                    m = mn;
+                    l *= f;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) { sum[k].x *= f; sum[k].y *= f; }
+                    // (the weights of the first half may have been taken by now: O holds them once that P V is done)
+                    if (c > 0) wait(kPVHalf + s, i & 1);
+                    if (i > 0 || c > 0) {
+                        fence_after();
+#pragma unroll 1
+                        for (int k = 0; k < D; k += 8) scale_o(to + k, f);
+                    }
+                }
+                base = m == -INFINITY ? 0.f : -m;
+                weights(c, v);
+                if (c == 0) tmem_ld32(ts + 64, v);
+                weights(c + 32, w);
+                if (c == 0) tmem_ld32(ts + 96, w);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar(kPReady + 2 * s + (c >> 6)));  // half of the weights
+                if (lane == 0) mbar_arrive(bar(kPReady + 2 * s + (c >> 6)));
             }
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         }
