@@ -15,17 +15,17 @@
 // 128 or 256 rows is what makes dense float16 operands affordable (the decode kernel for a few rows folds
 // the scales into its queries instead).
 //
-// The reference maximum m of a row moves only when 32 scores exceed it by more than 2^8 (weights up to
-// 256 cannot overflow float16, sums are float32): O and the weights already written are then rescaled by
-// the row's own thread. That S of step i + 1 is complete implies that P V of step i is (MMAs of one
-// thread complete in order), so no further wait is needed.
+// The reference maximum m of a row moves only when one of 64 scores exceeds it by more than 2^8 (weights up to
+// 256 cannot overflow float16, sums are float32): O, with the weights of the tokens before, is then rescaled by
+// the row's own thread. That S of step i + 1 is complete implies that P V of step i is (MMAs of one thread
+// complete in order), so only the second half of a tile waits for more (P V of the first).
 //
 // Measured at 4 bits in bfloat16: 256 query rows of each of 8 kv heads behind 32K tokens, 18 splits, 50 us; 8192 rows
-// behind 8K tokens, 340 us = 0.81 PFLOP/s, 49 % of the measured bfloat16 rate. A pair of row tiles takes
+// behind 8K tokens, 340 us = 0.82 PFLOP/s, 49 % of the measured bfloat16 rate. A pair of row tiles takes
 // about 4300 clocks a token tile, against 2048 for the MMAs, 2048 for the exponentials (16 a clock), 1000 for
-// HBM and about 2400 of instruction issue: what bounds it is the chain of one stream (scores 700, their
-// shared-memory operands being as long as the MMAs; weights 2600 to 3000 beside the other stream's and the
-// decoding warps; the last half of the output 240; hand-overs 600), of which two run side by side.
+// HBM and about 2400 of instruction issue: what bounds it is the chain of one stream (1000 until scores are
+// there: the last half of P V 256, Q K 700; weights 3350, of which about 2000 beside the other stream's), of
+// which two run side by side.
 //
 // Every wait is bounded; a role that gives up raises a flag (reported by vq_kivi_attend_status), leaves its
 // loop, and the CTA still waits (bounded) for its MMAs and frees its tensor memory.
