@@ -642,7 +642,8 @@ typedef struct vq_shared_attend_args {
     void *workspace;          /* >= vq_kivi_shared_attend_workspace_bytes(args), 16-byte aligned */
     int64_t workspace_bytes;
     int32_t variant;          /* 0 = choose by size; 1 = warp tiles for both parts; 2 = the tcgen05 kernel for
-                                 the prefix (and for own tokens with more than 32 query rows a kv head) */
+                                 the prefix (and for own tokens with more than 32 query rows a kv head), which
+                                 needs a positive scale */
     int32_t n_splits;         /* token splits of the prefix (at most 64); 0 = choose */
 } vq_shared_attend_args;
 int64_t vq_kivi_shared_attend_workspace_bytes(const vq_shared_attend_args *args);

@@ -583,12 +583,13 @@ int32_t plan_of(const vq_shared_attend_args &a, const DeviceInfo &di, Plan *out)
     // takes 5 us longer to start and end. Measured with 8 kv heads, warp tiles / tcgen05 in us: 64 rows
     // behind 1K tokens 10.3 / 12.2, 2K 13.9 / 12.8, 8K 28.7 / 16.7; 256 behind 512: 18.6 / 15.6; 32 behind 2K
     // 9.6 / 12.4, 4K 11.8 / 13.4, 8K 19.6 / 16.1; 16 behind 32K 27.1 / 30.3; own tokens, 1 request of 256 rows
-    // over 662: 22.5 / 16.7; 8 of 36 over 662: 26.5 / 19.9. It takes scales that are not negative.
+    // over 662: 22.5 / 16.7; 8 of 36 over 662: 26.5 / 19.9. It masks scores before it multiplies them, so it takes
+    // positive scales alone (-inf * 0 is NaN; the warp tiles mask the product).
     auto pays = [&](int64_t units, int64_t rows, const vq_kivi_rows &st) {
         return rows >= 32 && (double)units * (double)rows * ((double)st.n_quant + st.n_res) >= (rows < 64 && units < 32 ? 2 << 20 : 1 << 20);
     };
-    const bool can = a.scale >= 0.f;
-    VQ_REQUIRE(a.variant != 2 || (can && ip), VQ_ERR_SHAPE, "vq_kivi_shared_attend: the tcgen05 kernel needs a prefix and a scale that is not negative");
+    const bool can = a.scale * 1.4426950408889634f > 0.f;
+    VQ_REQUIRE(a.variant != 2 || (can && ip), VQ_ERR_SHAPE, "vq_kivi_shared_attend: the tcgen05 kernel needs a prefix and a positive scale");
     const int64_t units = (int64_t)a.B * a.H_kv;
     const bool prefix_tc5 = can && ip && (a.variant == 2 || (a.variant == 0 && pays(a.H_kv, all, pre)));
     const bool own_tc5 = can && io && (a.variant == 2 ? per_req > 32 : a.variant == 0 && pays(units, per_req, own));

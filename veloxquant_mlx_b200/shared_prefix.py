@@ -132,7 +132,8 @@ def kivi_shared_prefix_attend(q: torch.Tensor, prefix: KiviRows, own: KiviRows |
 
     The prefix is read once for all query rows of a kv head. Decoded keys and values, the exact rows and q
     enter the tensor cores as float16 (so they must lie within +-65504, also in bfloat16), softmax and sums are
-    float32. ``variant`` 1 / 2 force the warp-tile / the tensor-memory kernel for the prefix. Not differentiable.
+    float32. ``variant`` 1 / 2 force the warp-tile / the tensor-memory kernel for the prefix (2: ``scale`` > 0). Not
+    differentiable.
     """
     fn = "kivi_shared_prefix_attend"
     if q.ndim != 4:
