@@ -33,11 +33,24 @@ def _empty(x: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
-def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None) -> tuple[torch.Tensor, float]:
+_BASE = 10000.0
+# What each kind of scaling takes beside its name and the base; the second set says nothing about the frequencies.
+_SCALING_KEYS = {
+    "default": set(),
+    "linear": {"factor"},
+    "ntk": {"factor"},
+    "llama3": {"factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"},
+    "yarn": {"factor", "original_max_position_embeddings", "attention_factor", "beta_fast", "beta_slow", "mscale", "mscale_all_dim", "truncate"},
+}
+_NO_EFFECT = {"rope_type", "type", "rope_theta", "original_max_position_embeddings", "max_position_embeddings", "finetuned"}
+
+
+def rotary_frequencies(rotary_dim: int, base: float | None = None, scaling: dict | None = None) -> tuple[torch.Tensor, float]:
     """Angle per position of each of the ``rotary_dim / 2`` pairs (float64, on the host) and the
     factor on sine and cosine.
 
-    Without ``scaling``: ``base ** (-2 i / rotary_dim)`` and 1. ``scaling["rope_type"]`` is one of
+    Without ``scaling``: ``base ** (-2 i / rotary_dim)`` and 1. ``base`` defaults to ``scaling["rope_theta"]``, or to
+    10000; one that contradicts ``rope_theta`` is refused. ``scaling["rope_type"]`` is one of
 
     * ``"default"``;
     * ``"linear"``: every frequency divided by ``factor``;
@@ -48,16 +61,29 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     * ``"yarn"``: the same between the pairs that make ``beta_slow`` (1) and ``beta_fast`` (32) turns
       over the original context, the ramp linear in the pair's index (rounded outwards unless
       ``truncate`` is false); the factor on sine and cosine is ``attention_factor``, by default
-      ``0.1 ln(factor) + 1``.
+      ``m(mscale) / m(mscale_all_dim)`` where both are given (and not 0), else ``m(1)``, with
+      ``m(x) = 0.1 x ln(factor) + 1`` (1 for a factor of at most 1).
+
+    A key that is None counts as absent; one that the kind does not know is refused, so that nothing that would change
+    the frequencies is passed over (``partial_rotary_factor`` is the business of :class:`RotaryEmbedding`).
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_frequencies: rotary_dim={rotary_dim} must be even and at least 2")
+    scaling = {name: x for name, x in (scaling or {}).items() if x is not None}
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind not in _SCALING_KEYS:
+        raise ValueError(f"rotary_frequencies: unknown rope_type {kind!r}")
+    unknown = sorted(str(name) for name in scaling if name not in _SCALING_KEYS[kind] and name not in _NO_EFFECT)
+    if unknown:
+        raise ValueError(f"rotary_frequencies: rope_type {kind!r} does not take {', '.join(map(repr, unknown))}")
+    theta = scaling.get("rope_theta")
+    if base is None:
+        base = _BASE if theta is None else float(theta)
+    elif theta is not None and float(theta) != float(base):
+        raise ValueError(f"rotary_frequencies: base={base} contradicts rope_theta={theta}")
     if not base > 0:
         raise ValueError(f"rotary_frequencies: base={base} must be positive")
     pair = torch.arange(rotary_dim // 2, dtype=torch.float64)
-    kind = "default" if not scaling else scaling.get("rope_type", scaling.get("type", "default"))
-    if kind not in ("default", "linear", "ntk", "llama3", "yarn"):
-        raise ValueError(f"rotary_frequencies: unknown rope_type {kind!r}")
 
     def need(name):
         if name not in scaling:
@@ -77,6 +103,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     if kind == "linear":
         return freq / factor, 1.0
     old = need("original_max_position_embeddings")
+    if not old > 0:
+        raise ValueError(f"rotary_frequencies: original_max_position_embeddings={old} must be positive")
     if kind == "llama3":
         lo, hi = need("low_freq_factor"), need("high_freq_factor")
         if not hi > lo:
@@ -86,6 +114,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
         return freq * (keep + (1.0 - keep) / factor), 1.0
     # yarn: the index of the pair that makes n turns over the original context
     fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+    if not (fast > 0 and slow > 0 and base != 1):
+        raise ValueError(f"rotary_frequencies: beta_fast={fast} and beta_slow={slow} must be positive, base={base} other than 1")
     at = lambda n: rotary_dim * math.log(old / (n * 2.0 * math.pi)) / (2.0 * math.log(base))  # noqa: E731
     lo, hi = at(fast), at(slow)
     if scaling.get("truncate", True):
@@ -94,8 +124,13 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     if hi == lo:
         hi += 0.001
     stretched = ((pair - lo) / (hi - lo)).clamp(0.0, 1.0)
-    att = scaling.get("attention_factor")
-    att = float(att) if att is not None else (0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0)
+    m = lambda x: 0.1 * x * math.log(factor) + 1.0 if factor > 1.0 else 1.0  # noqa: E731
+    if "attention_factor" in scaling:
+        att = float(scaling["attention_factor"])
+    elif scaling.get("mscale") and scaling.get("mscale_all_dim"):
+        att = m(float(scaling["mscale"])) / m(float(scaling["mscale_all_dim"]))
+    else:
+        att = m(1.0)
     return freq * ((1.0 - stretched) + stretched / factor), att
 
 
@@ -106,7 +141,8 @@ class RotaryEmbedding:
     pairs ``(c, c + rotary_dim/2)`` (``layout="half"``) or ``(2c, 2c+1)`` (``"interleaved"``).
     The frequencies are :func:`rotary_frequencies` of ``base`` and ``scaling``, or ``inv_freq``
     (``[rotary_dim/2]``, angle per position, taken in float64); ``attention_factor`` overrides the
-    factor on sine and cosine.
+    factor on sine and cosine. ``scaling["partial_rotary_factor"]`` stands for
+    ``rotary_dim = int(head_dim * factor)``; a ``rotary_dim`` that contradicts it is refused.
 
     ``rope(q, k, positions)`` returns the turned ``q`` and ``k`` (``rope(q)`` one tensor) as new
     contiguous tensors: ``q [B, H_q, S, D]``, ``k [B, H_kv, S, D]`` in float16, bfloat16 or float32
@@ -122,8 +158,14 @@ class RotaryEmbedding:
     holds: no graph that an earlier eager pass built over the same leaves may still be alive.
     """
 
-    def __init__(self, head_dim: int, *, rotary_dim: int | None = None, base: float = 10000.0, layout: str = "half",
+    def __init__(self, head_dim: int, *, rotary_dim: int | None = None, base: float | None = None, layout: str = "half",
                  scaling: dict | None = None, inv_freq: Any = None, attention_factor: float | None = None, device=None) -> None:
+        part = scaling.get("partial_rotary_factor") if scaling else None
+        if part is not None:
+            scaling = {name: x for name, x in scaling.items() if name != "partial_rotary_factor"}
+            if rotary_dim is not None and int(rotary_dim) != int(head_dim * part):
+                raise ValueError(f"RotaryEmbedding: rotary_dim={rotary_dim} contradicts partial_rotary_factor={part} of head_dim={head_dim}")
+            rotary_dim = int(head_dim * part)
         rotary_dim = head_dim if rotary_dim is None else int(rotary_dim)
         if head_dim < 2 or rotary_dim < 2 or rotary_dim > head_dim or rotary_dim % 2:
             raise ValueError(f"RotaryEmbedding: rotary_dim={rotary_dim} must be even and in 2..head_dim={head_dim}")
