@@ -15,6 +15,7 @@ import math
 from typing import Any
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import _DTYPE_CODE as _DTYPE_CODES
@@ -151,7 +152,8 @@ class RotaryEmbedding:
     0, the others following (default 0). ``inverse=True`` turns the other way, times the same
     ``attention_factor``: the gradient. Products are float32, angles float64 (exact
     to float32 for positions up to 2**31 and beyond); one rounding to the tensors' type at the end.
-    Gradients flow to ``q`` and ``k`` (also twice), not to positions or frequencies.
+    Derivatives flow through ``q`` and ``k`` in reverse mode (also twice) and forward mode
+    (``torch.autograd.forward_ad``), not through positions or frequencies.
 
     The frequency table is put on a device at its first use there; make that use (or pass
     ``device=``) before a CUDA-graph capture. Where a backward pass is captured, PyTorch's own rule
@@ -287,7 +289,7 @@ class RotaryEmbedding:
     def __call__(self, q: torch.Tensor, k: torch.Tensor | None = None, positions=None, *, inverse: bool = False):
         fn = "RotaryEmbedding"
         self._check(fn, q, k)
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        if forward_ad._current_level >= 0 or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
             out = _Rotate.apply(self, positions, inverse, q, k)
         else:
             out = self._rotate(fn, q, k, positions, inverse)
@@ -357,7 +359,8 @@ def _turn(rope, positions, inverse, q, k):
 
 
 class _Rotate(torch.autograd.Function):
-    """The turn as a differentiable operation: linear in q and k, its gradient is the inverse turn."""
+    """The turn as a differentiable operation: linear in q and k, its gradient is the inverse turn, its derivative along a
+    direction the direction's own turn."""
 
     @staticmethod
     def forward(ctx, rope, positions, inverse, q, k):
@@ -368,15 +371,30 @@ class _Rotate(torch.autograd.Function):
             ctx.save_for_backward(positions)
         else:
             ctx.positions = positions
-        return _turn(rope, positions, inverse, q, k)
+        out = _turn(rope, positions, inverse, q, k)
+        if forward_ad._current_level >= 0:
+            ctx.tangent_positions = positions
+            ctx.like = [None if y is None else (y.shape, y.dtype, y.device) for y in out]
+        return out
+
+    @staticmethod
+    def jvp(ctx, _rope, _positions, _inverse, tq, tk):
+        shapes, positions = ctx.like, ctx.tangent_positions
+        # (a tangent may be torch's placeholder for zeros, which has no memory)
+        tq, tk = (t.clone() if t is not None and t._is_zerotensor() else t for t in (tq, tk))
+        if tq is not None:
+            tq, tk = _Rotate.apply(ctx.rope, positions, ctx.inverse, tq, tk)
+        elif tk is not None:
+            tk = _Rotate.apply(ctx.rope, positions, ctx.inverse, tk, None)[0]
+        return tuple(torch.zeros(like[0], dtype=like[1], device=like[2]) if t is None and like is not None else t for t, like in zip((tq, tk), shapes))
 
     @staticmethod
     def backward(ctx, gq, gk):
         positions = ctx.saved_tensors[0] if ctx.tensor_positions else ctx.positions
         need_q, need_k = ctx.needs_input_grad[3], ctx.needs_input_grad[4]
         gq, gk = gq if need_q else None, gk if need_k else None
-        # (through the function again only where a second derivative may be asked for)
-        turn = _Rotate.apply if torch.is_grad_enabled() else _turn
+        # (through the function again only where a second derivative may be asked for, in either mode)
+        turn = _Rotate.apply if torch.is_grad_enabled() or forward_ad._current_level >= 0 else _turn
         if gq is not None:
             gq, gk = turn(ctx.rope, positions, not ctx.inverse, gq, gk)
         elif gk is not None:
