@@ -12,6 +12,7 @@ import struct
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libvqb200.so")
@@ -327,6 +328,17 @@ def on_device(device: torch.device):
     if idx is None or idx == torch.cuda.current_device():
         return _NO_GUARD
     return torch.cuda.device(idx)
+
+
+def carries_derivative(*tensors) -> bool:
+    """Whether a derivative, in reverse or forward mode, is asked for through one of ``tensors`` (None: not given)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level >= 0:
+        return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return False
 
 
 def require_cuda(t: torch.Tensor, name: str) -> None:

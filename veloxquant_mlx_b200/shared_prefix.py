@@ -96,6 +96,7 @@ class KiviRows:
         self.batch, self.heads, self.head_dim, self.store_bits, self.device = B, H, D, store_bits, first.device
         self._cap, self._cap_res, self._pointers, self._strides = cap, cap_res, pointers, (*strides, res_stride)
         self._tensors = (k_codes, k_scale, k_zero, v_codes, v_scale, v_zero, k_res, v_res)  # (kept alive)
+        self._floats = [t for t in self._tensors if t is not None and t is not k_codes and t is not v_codes]
         self._k_res_ptr, self._v_res_ptr = (0, 0) if k_res is None else (k_res.data_ptr(), v_res.data_ptr())
         self.resize(cap // _GROUP * _GROUP if n_quant is None else n_quant, cap_res - res_offset if n_res is None else n_res, res_offset)
 
@@ -133,7 +134,7 @@ def kivi_shared_prefix_attend(q: torch.Tensor, prefix: KiviRows, own: KiviRows |
     The prefix is read once for all query rows of a kv head. Decoded keys and values, the exact rows and q
     enter the tensor cores as float16 (so they must lie within +-65504, also in bfloat16), softmax and sums are
     float32. ``variant`` 1 / 2 force the warp-tile / the tensor-memory kernel for the prefix (2: ``scale`` > 0). Not
-    differentiable.
+    differentiable: tensors that carry a derivative (either mode) are refused.
     """
     fn = "kivi_shared_prefix_attend"
     if q.ndim != 4:
@@ -165,8 +166,8 @@ def kivi_shared_prefix_attend(q: torch.Tensor, prefix: KiviRows, own: KiviRows |
     if own_start is not None:
         if own_start.dtype is not torch.int32 or tuple(own_start.shape) != (B,) or own_start.device != dev or not own_start.is_contiguous():
             raise ValueError(f"{fn}: own_start must be a contiguous int32 [{B}] tensor on {dev}, got {own_start.dtype} {tuple(own_start.shape)}")
-    if q.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{fn}: not differentiable (q requires grad; call it under torch.no_grad())")
+    if _lib.carries_derivative(q, *prefix._floats, *(() if own is None else own._floats)):
+        raise ValueError(f"{fn}: not differentiable (q, exact rows, scales or zeros carry a derivative; call it under torch.no_grad())")
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=dev)
     elif out.shape != q.shape or out.dtype is not dt or out.device != dev or not out.is_contiguous():
