@@ -713,50 +713,55 @@ class KIVIKVCache(StandaloneProtocol):
             self._dtype = keys.dtype
         self._shape_bhd = (B, H, D)
         dev = keys.device
+        uncounted = self.offset - self._n_quantized - self._n_res
         self.offset += S
         new_boundary = self._quantization_boundary()
         n_flush = new_boundary - self._n_quantized
         self._just_flushed = n_flush > 0
-        if n_flush <= 0:
-            self._make_room(B, H, D, S, dev, keys.dtype)
-            store(keys, values, S, overlap_previous)
-        elif self._n_res == 0:
-            # A (prefill) block onto an empty residual: its head is quantized straight from the
-            # caller's tensor, only its tail is copied into the residual buffer.
-            self._ensure_capacity(B, H, D, new_boundary, dev, keys.dtype)
-            self._quantize_rows(keys, values, n_flush)
-            self._n_quantized = new_boundary
-            keep = S - n_flush
-            self._res_lo = 0
-            self._ensure_residual(B, H, D, keep, dev, keys.dtype)
-            if keep > 0:
-                self._store_block(keys[:, :, n_flush:], values[:, :, n_flush:], keep)
-        elif S <= self._residual_length + self._group_size:
-            # Decode: the rows to flush are the oldest unquantized rows. The block is stored behind
-            # the live rows, then the aged rows are quantized where they lie and the window's
-            # start moves on: no concatenation, no shifting, no allocation.
-            self._make_room(B, H, D, S, dev, keys.dtype)
-            store(keys, values, S, False)
-            self._ensure_capacity(B, H, D, new_boundary, dev, keys.dtype)
-            lo = self._res_lo
-            self._quantize_rows(self._k_res[:, :, lo : lo + n_flush], self._v_res[:, :, lo : lo + n_flush], n_flush)
-            self._res_lo += n_flush
-            self._n_res -= n_flush
-            self._n_quantized = new_boundary
-        else:
-            # A long block onto a non-empty residual: the rows to flush span both.
-            lo = self._res_lo
-            src_k = torch.cat([self._k_res[:, :, lo : lo + self._n_res], keys], dim=2)
-            src_v = torch.cat([self._v_res[:, :, lo : lo + self._n_res], values], dim=2)
-            self._ensure_capacity(B, H, D, new_boundary, dev, keys.dtype)
-            self._quantize_rows(src_k, src_v, n_flush)
-            keep = src_k.shape[2] - n_flush
-            self._n_res = 0
-            self._res_lo = 0
-            self._ensure_residual(B, H, D, keep, dev, keys.dtype)
-            if keep > 0:
-                self._store_block(src_k[:, :, n_flush:], src_v[:, :, n_flush:], keep)
-            self._n_quantized = new_boundary
+        try:
+            if n_flush <= 0:
+                self._make_room(B, H, D, S, dev, keys.dtype)
+                store(keys, values, S, overlap_previous)
+            elif self._n_res == 0:
+                # A (prefill) block onto an empty residual: its head is quantized straight from the
+                # caller's tensor, only its tail is copied into the residual buffer.
+                self._ensure_capacity(B, H, D, new_boundary, dev, keys.dtype)
+                self._quantize_rows(keys, values, n_flush)
+                self._n_quantized = new_boundary
+                keep = S - n_flush
+                self._res_lo = 0
+                self._ensure_residual(B, H, D, keep, dev, keys.dtype)
+                if keep > 0:
+                    self._store_block(keys[:, :, n_flush:], values[:, :, n_flush:], keep)
+            elif S <= self._residual_length + self._group_size:
+                # Decode: the rows to flush are the oldest unquantized rows. The block is stored behind
+                # the live rows, then the aged rows are quantized where they lie and the window's
+                # start moves on: no concatenation, no shifting, no allocation.
+                self._make_room(B, H, D, S, dev, keys.dtype)
+                store(keys, values, S, False)
+                self._ensure_capacity(B, H, D, new_boundary, dev, keys.dtype)
+                lo = self._res_lo
+                self._quantize_rows(self._k_res[:, :, lo : lo + n_flush], self._v_res[:, :, lo : lo + n_flush], n_flush)
+                self._res_lo += n_flush
+                self._n_res -= n_flush
+                self._n_quantized = new_boundary
+            else:
+                # A long block onto a non-empty residual: the rows to flush span both.
+                lo = self._res_lo
+                src_k = torch.cat([self._k_res[:, :, lo : lo + self._n_res], keys], dim=2)
+                src_v = torch.cat([self._v_res[:, :, lo : lo + self._n_res], values], dim=2)
+                self._ensure_capacity(B, H, D, new_boundary, dev, keys.dtype)
+                self._quantize_rows(src_k, src_v, n_flush)
+                keep = src_k.shape[2] - n_flush
+                self._n_res = 0
+                self._res_lo = 0
+                self._ensure_residual(B, H, D, keep, dev, keys.dtype)
+                if keep > 0:
+                    self._store_block(src_k[:, :, n_flush:], src_v[:, :, n_flush:], keep)
+                self._n_quantized = new_boundary
+        except BaseException:   # a refused block is not counted: the offset is what the rows held say
+            self.offset = self._n_quantized + self._n_res + uncounted
+            raise
         self._account_bytes(B, H, S, D, max(n_flush, 0))
         if (S == 1 and keys.dtype is self._k_res.dtype and keys.is_cuda and (D * keys.element_size()) % 16 == 0
                 and torch.cuda.current_device() == keys.device.index):
@@ -776,7 +781,9 @@ class KIVIKVCache(StandaloneProtocol):
         :class:`rotary.RotaryEmbedding`) and append the rotated keys and ``values``: ``(rotated q,
         *update_and_fetch(rotated keys, values))``. ``positions``: as in the embedding; by default the
         tokens follow the cached ones. A block that goes through the residual window (every decode
-        step) is rotated straight into it, in one launch; a prompt is rotated first."""
+        step) is rotated straight into it, in one launch; a prompt, and a block with derivatives, is rotated first.
+        The rotated ``q`` is differentiable, what the cache holds is not. A refused call leaves the cache's tokens
+        as they were."""
         if positions is None:
             positions = int(self.offset)
         if (type(self).update_and_fetch is KIVIKVCache.update_and_fetch and q.ndim == 4 and keys.ndim == 4 and keys.shape == values.shape
@@ -784,8 +791,8 @@ class KIVIKVCache(StandaloneProtocol):
                                                                                   and self._k_res.shape[:2] == keys.shape[:2]))):
             S, g = keys.shape[2], self._group_size
             aged = max(0, self.offset + S - self._residual_length) // g * g > self._n_quantized
-            if S and (not aged or (self._n_res and S <= self._residual_length + g)):
-                rope._check_append(q, keys, values)   # (before the cache's counters move)
+            if S and (not aged or (self._n_res and S <= self._residual_length + g)) and not _lib.carries_derivative(q, keys, values):
+                rope._check_append(q, keys, values)   # (before buffers are made or moved)
                 rope._positions("KIVIKVCache.update_rotary", positions, keys.shape[0], S, keys.device)
                 turned = []
 
@@ -796,7 +803,7 @@ class KIVIKVCache(StandaloneProtocol):
                 out = self._append_block(keys, values, False, store)
                 return (turned[0], *out)
         q2, k2 = rope(q, keys, positions)
-        return (q2, *self.update_and_fetch(k2, values))
+        return (q2, *self.update_and_fetch(k2.detach(), values.detach()))
 
     def _live_res(self):
         lo = self._res_lo
