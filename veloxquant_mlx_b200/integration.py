@@ -141,9 +141,9 @@ def make_cache_layer_class():
 
         ``update`` appends through ``update_and_fetch``. A standard-mode cache returns the
         history as it would be after dequantization, which any attention implementation can
-        consume; a memory-bound cache returns zero-length sentinels that carry a reference to
-        the cache (``keys.velox_cache``), and ``veloxquant_attention`` attends over the packed
-        store instead.
+        consume; a memory-bound cache returns zero-length sentinels without channels that carry a
+        reference to the cache (``keys.velox_cache``), and ``veloxquant_attention`` attends over the
+        packed store instead (any other attention function fails on them).
         """
 
         is_compileable = False
@@ -162,7 +162,10 @@ def make_cache_layer_class():
                 self.lazy_initialization(key_states, value_states)
             k, v = self.cache.update_and_fetch(key_states, value_states)
             if getattr(self.cache, "_memory_bound", False):
-                k = k.view(k.shape)  # a fresh tensor object: the attribute must not leak between layers
+                # A fresh tensor object (the attribute must not leak between layers), and no channels: dense
+                # attention over zero-length keys of the right width gives zeros without an error, so a model that
+                # was not routed to veloxquant_attention has to fail here.
+                k, v = k[..., :0], v[..., :0]
                 k.velox_cache = self.cache
             self.keys, self.values = k, v
             return k, v
@@ -216,12 +219,18 @@ def fork_hf_cache(cache: Any, batch: int):
     """A ``transformers.Cache`` for ``batch`` requests that continue one prefilled prompt: ``cache`` is a
     cache of :func:`make_hf_cache` (method ``kivi``) after the prompt ran through the model at batch 1.
     Its layers' packed prompt is shared, not copied; every layer of the result is a
-    ``shared_prefix.SharedPrefixKIVICache`` (attend with :func:`veloxquant_attention`)."""
+    ``shared_prefix.SharedPrefixKIVICache``, memory-bound whatever the prompt's cache was: the model has to attend
+    with :func:`veloxquant_attention` (:func:`patch_hf_for_fused_sdpa`), any other attention fails. The requests'
+    next tokens must be of one length, without a padding mask; padded batches go through the caches themselves
+    (``SharedPrefixKIVICache.set_own_start``)."""
     from transformers.cache_utils import Cache
 
     from .shared_prefix import SharedPrefixKIVICache
 
     Layer = make_cache_layer_class()
+    for i, layer in enumerate(cache.layers):
+        if not isinstance(layer, Layer):
+            raise ValueError(f"fork_hf_cache: layer {i} is a {type(layer).__name__}, not one of make_hf_cache")
     return Cache(layers=[Layer(SharedPrefixKIVICache(layer.cache, batch)) for layer in cache.layers])
 
 
