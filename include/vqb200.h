@@ -627,7 +627,11 @@ typedef struct vq_kivi_rows {
  * with VQ_ATTEND_CAUSAL, t <= n - S_q + r. A row that sees nothing gives zeros (and lse -inf).
  * float16 or bfloat16; D 64 or 128, group 32, store_bits 2, 4 or 8. Decoded keys and values
  * enter the tensor cores as float16 (also for bfloat16 queries), so scale, zero, code*scale+zero, the
- * exact rows and q must lie within +-65504. Up to three launches: tcgen05 tiles, warp tiles, merge. */
+ * exact rows and q must lie within +-65504, and small ones lose bits that bfloat16 would keep: a key
+ * or value is off by up to 2^-11 of itself or, below 2^-14, by 2^-25. For bfloat16 at 2 and 4 bits scale and
+ * zero are float16 too: off by up to 2^-11 (code*scale + |zero| + |value|) and 2^-20 absolute, so values
+ * below about 2^-12 lose accuracy (relative rms error of the output at 4 bits for values around 1 / 1e-4 /
+ * 1e-5 / 1e-6: 0.2 / 0.2 / 1.3 / 14 %; bfloat16's own rounding is 0.17 %). Up to three launches: tcgen05 tiles, warp tiles, merge. */
 typedef struct vq_shared_attend_args {
     const void *q;            /* [B, H_q, S_q, D] contiguous */
     void *out;                /* [B, H_q, S_q, D] contiguous, dtype of q */

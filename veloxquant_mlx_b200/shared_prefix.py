@@ -132,8 +132,9 @@ def kivi_shared_prefix_attend(q: torch.Tensor, prefix: KiviRows, own: KiviRows |
     that sees nothing gives zeros and ``lse`` -inf.
 
     The prefix is read once for all query rows of a kv head. Decoded keys and values, the exact rows and q
-    enter the tensor cores as float16 (so they must lie within +-65504, also in bfloat16), softmax and sums are
-    float32. ``variant`` 1 / 2 force the warp-tile / the tensor-memory kernel for the prefix (2: ``scale`` > 0). Not
+    enter the tensor cores as float16 also for bfloat16 (so they must lie within +-65504; small ones keep 2^-25 absolute, and
+    decoded bfloat16 ones of 2 and 4 bits 2^-20: bfloat16 values below about 2^-12 lose accuracy, 1.3 % at 1e-5, 14 % at
+    1e-6), softmax and sums are float32. ``variant`` 1 / 2 force the warp-tile / the tensor-memory kernel for the prefix (2: ``scale`` > 0). Not
     differentiable: tensors that carry a derivative (either mode) are refused.
     """
     fn = "kivi_shared_prefix_attend"
