@@ -21,6 +21,9 @@ constexpr int kGroup = 32;
 constexpr int kExact = 12;  // exact rows of one work item: as many bytes as a packed group of 4-bit codes
 constexpr int kWarps = 4;
 constexpr int kStages = 2;
+// Weights, at most 1, are held times 2^15: float16's smallest step then is 2^-39 of the row's largest weight
+// instead of 2^-24, so that many tokens behind one that outweighs them are not lost. The factor is in the exponent.
+constexpr float kLift = 15.f;
 
 struct RowsParams {
     const void *q;
@@ -249,14 +252,15 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
                         mx[c & 1] = fmaxf(mx[c & 1], s[nt][k][c]);
                     }
             }
-            float base[2], f[2];
+            float low[2], f[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], d));
                 const float mn = fmaxf(m[nt][i], mx[i]);
-                base[i] = mn == -INFINITY ? 0.f : mn;
-                f[i] = ex2(m[nt][i] - base[i]);
+                const float base = mn == -INFINITY ? 0.f : mn;
+                f[i] = ex2(m[nt][i] - base);
+                low[i] = base - kLift;
                 m[nt][i] = mn;
                 l[nt][i] *= f[i];
             }
@@ -269,7 +273,7 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
                 float e[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    e[c] = ex2(s[nt][k][c] - base[c & 1]);
+                    e[c] = ex2(s[nt][k][c] - low[c & 1]);
                     l[nt][c & 1] += e[c];
                 }
                 pb[nt][k][0] = transpose8x8(pack_f16(e[0], e[1]));
@@ -450,7 +454,7 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], d);
             const int r = 8 * nt + 2 * c4 + i;
-            if (g8 == 0) { sh_m[warp][r] = m[nt][i]; sh_l[warp][r] = l[nt][i]; }
+            if (g8 == 0) { sh_m[warp][r] = m[nt][i] - kLift; sh_l[warp][r] = l[nt][i]; }  // (l and o are 2^kLift times those of m)
             float *dst = sh_o + (warp * ROWS + r) * LD + g8 * CN;
 #pragma unroll
             for (int j = 0; j < MT; ++j) *reinterpret_cast<float2 *>(dst + 2 * j) = make_float2(o[nt][j][i], o[nt][j][2 + i]);

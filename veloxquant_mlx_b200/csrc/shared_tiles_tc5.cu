@@ -15,9 +15,11 @@
 // 128 or 256 rows is what makes dense float16 operands affordable (the decode kernel for a few rows folds
 // the scales into its queries instead).
 //
-// The reference maximum m of a row moves only when one of 64 scores exceeds it by more than 2^8 (weights up to
-// 256 cannot overflow float16, sums are float32): O, with the weights of the tokens before, is then rescaled by
-// the row's own thread. That S of step i + 1 is complete implies that P V of step i is (MMAs of one thread
+// The reference maximum m of a row moves only when one of 64 scores exceeds it by more than 2^8: O, with the weights of
+// the tokens before, is then rescaled by the row's own thread. Weights are held times 2^7: up to 2^15, which float16
+// holds, and down to 2^-32 of 2^m before its smallest step (2^-25 without the factor, and then the tail behind one
+// token that outweighs all others is lost: 4096 tokens of 2^-26 each came out as 0). The factor costs nothing: it is in
+// the exponent, and leaves with m. That S of step i + 1 is complete implies that P V of step i is (MMAs of one thread
 // complete in order), so only the second half of a tile waits for more (P V of the first).
 //
 // Measured at 4 bits in bfloat16: 256 query rows of each of 8 kv heads behind 32K tokens, 18 splits, 50 us; 8192 rows
@@ -42,6 +44,7 @@ constexpr int kGroup = 32;
 constexpr int kThreads = 17 * 32;
 constexpr uint32_t kSpin = 1u << 20;
 constexpr float kLazy = 8.f;       // log2 of how far a maximum may rise before O is rescaled
+constexpr float kLift = 7.f;       // log2 of the factor on weights: kLazy + kLift = 15, below float16's 2^16
 
 __device__ int g_shared_timeout = 0;
 
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
                         for (int k = 0; k < D; k += 8) scale_o(to + k, f);
                     }
                 }
-                base = m == -INFINITY ? 0.f : -m;
+                base = m == -INFINITY ? 0.f : kLift - m;
                 weights(c, v);
                 if (c == 0) tmem_ld32(ts + 64, v);
                 weights(c + 32, w);
@@ -396,6 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
             }
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         }
+        m -= kLift;  // (O and l are 2^kLift times those of m)
         // O goes out through shared memory: a row a lane there, whole rows at a time to global memory. The
         // tiles it overwrites are done with when both streams are.
         if (n_steps > 0) wait(kODone, 0);
