@@ -13,6 +13,7 @@ from __future__ import annotations
 from typing import Any
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import KIVI_ROWS_PACK, SHARED_ATTEND_HEAD, SHARED_ATTEND_TAIL, check, lib, require_cuda, stream_ptr
@@ -96,7 +97,7 @@ class KiviRows:
         self.batch, self.heads, self.head_dim, self.store_bits, self.device = B, H, D, store_bits, first.device
         self._cap, self._cap_res, self._pointers, self._strides = cap, cap_res, pointers, (*strides, res_stride)
         self._tensors = (k_codes, k_scale, k_zero, v_codes, v_scale, v_zero, k_res, v_res)  # (kept alive)
-        self._floats = [t for t in self._tensors if t is not None and t is not k_codes and t is not v_codes]
+        self._grad = any(t is not None and t.requires_grad for t in self._tensors)
         self._k_res_ptr, self._v_res_ptr = (0, 0) if k_res is None else (k_res.data_ptr(), v_res.data_ptr())
         self.resize(cap // _GROUP * _GROUP if n_quant is None else n_quant, cap_res - res_offset if n_res is None else n_res, res_offset)
 
@@ -167,7 +168,8 @@ def kivi_shared_prefix_attend(q: torch.Tensor, prefix: KiviRows, own: KiviRows |
     if own_start is not None:
         if own_start.dtype is not torch.int32 or tuple(own_start.shape) != (B,) or own_start.device != dev or not own_start.is_contiguous():
             raise ValueError(f"{fn}: own_start must be a contiguous int32 [{B}] tensor on {dev}, got {own_start.dtype} {tuple(own_start.shape)}")
-    if _lib.carries_derivative(q, *prefix._floats, *(() if own is None else own._floats)):
+    if (torch.is_grad_enabled() and (q.requires_grad or prefix._grad or (own is not None and own._grad))) or (
+            forward_ad._current_level >= 0 and _lib.carries_derivative(q, *prefix._tensors, *(() if own is None else own._tensors))):
         raise ValueError(f"{fn}: not differentiable (q, exact rows, scales or zeros carry a derivative; call it under torch.no_grad())")
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=dev)
