@@ -559,6 +559,10 @@ class KIVIKVCache(StandaloneProtocol):
         self._residual_fp16_bytes = 0
         self._tokens_seen = 0
 
+    def __getstate__(self):
+        # the kept argument blocks hold addresses of this cache's buffers: a copy makes its own
+        return {**self.__dict__, "_attend_plan": None, "_append_plan": None, "_quant_args": None}
+
     # -- policy ------------------------------------------------------------------------
     def _quantization_boundary(self) -> int:
         aged = max(0, self.offset - self._residual_length)

@@ -110,10 +110,18 @@ class KiviRows:
         skip = res_offset * self.head_dim * 2
         res = (self._k_res_ptr + skip, self._v_res_ptr + skip) if n_res else (0, 0)
         self._args = KIVI_ROWS_PACK.pack(*self._pointers, *res, *self._strides, n_quant, n_res)
-        self.n_quant, self.n_res = n_quant, n_res
+        self.n_quant, self.n_res, self._res_offset = n_quant, n_res, res_offset
+
+    def __reduce__(self):
+        # (copies and pickles refer to their own tensors' memory, not to this object's)
+        return _rows_again, (self._tensors, self.store_bits, self.n_quant, self.n_res, self._res_offset)
 
     def __len__(self) -> int:
         return self.n_quant + self.n_res
+
+
+def _rows_again(tensors, store_bits, n_quant, n_res, res_offset):
+    return KiviRows(*tensors, store_bits=store_bits, n_quant=n_quant, n_res=n_res, res_offset=res_offset)
 
 
 _EMPTY = bytes(KIVI_ROWS_PACK.size)
