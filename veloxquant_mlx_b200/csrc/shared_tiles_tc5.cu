@@ -47,6 +47,8 @@ constexpr float kLazy = 8.f;       // log2 of how far a maximum may rise before 
 constexpr float kLift = 7.f;       // log2 of the factor on weights: kLazy + kLift = 15, below float16's 2^16
 
 __device__ int g_shared_timeout = 0;
+std::atomic<uint64_t> g_launched{0};  // one bit a device that the kernel was ever launched on (or captured for)
+uint64_t device_bit(int dev) { return 1ull << (dev & 63); }
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
@@ -724,6 +726,9 @@ int32_t launch(const TileParams &p, unsigned blocks, cudaStream_t st) {
     static std::atomic<uint64_t> allowed{0};
     const int32_t rc = allow_shared_memory(&shared_tiles_tc5_kernel<D, SB, T>, Layout<D>::BYTES, allowed);
     if (rc != VQ_OK) return rc;
+    int dev = 0;
+    VQ_CHECK_CUDA(cudaGetDevice(&dev));
+    if (!(g_launched.load(std::memory_order_relaxed) & device_bit(dev))) g_launched.fetch_or(device_bit(dev));
     shared_tiles_tc5_kernel<D, SB, T><<<blocks, kThreads, Layout<D>::BYTES, st>>>(p);
     VQ_CHECK_LAUNCH("shared_tiles_tc5_kernel");
     return VQ_OK;
@@ -805,10 +810,14 @@ int32_t shared_tiles_tc5_launch(const vq_shared_attend_args &a, const SharedPart
 }
 
 int32_t shared_tiles_tc5_take_timeout(int *flag) {
+    int dev = 0;
+    *flag = 0;
+    VQ_CHECK_CUDA(cudaGetDevice(&dev));
+    if (!(g_launched.load() & device_bit(dev))) return VQ_OK;  // (a status call costs those who never launch it nothing)
     VQ_CHECK_CUDA(cudaDeviceSynchronize());
     const int zero = 0;
     VQ_CHECK_CUDA(cudaMemcpyFromSymbol(flag, g_shared_timeout, sizeof(int)));
-    VQ_CHECK_CUDA(cudaMemcpyToSymbol(g_shared_timeout, &zero, sizeof(int)));
+    if (*flag) VQ_CHECK_CUDA(cudaMemcpyToSymbol(g_shared_timeout, &zero, sizeof(int)));
     return VQ_OK;
 }
 
