@@ -85,3 +85,15 @@ def test_part_of_the_head_by_its_factor():
         RotaryEmbedding(128, scaling=part, rotary_dim=64)
     with pytest.raises(ValueError, match="rotary_dim"):
         RotaryEmbedding(128, scaling={"partial_rotary_factor": 1.5})
+
+
+@pytest.mark.parametrize("kind", ["float64 tensor", "float64 array"])
+def test_given_frequencies_are_the_embedding_s_own(kind):
+    import numpy as np
+
+    given = torch.linspace(1, 0.1, 8, dtype=torch.float64) if kind == "float64 tensor" else np.linspace(1, 0.1, 8)
+    rope, want = RotaryEmbedding(16, inv_freq=given), torch.as_tensor(given).clone()
+    given *= 0  # the caller's buffer is used again
+    assert torch.equal(rope.inv_freq, want)
+    rope.inv_freq.zero_()  # and what the property gives is a copy
+    assert torch.equal(rope.inv_freq, want)

@@ -178,7 +178,7 @@ class RotaryEmbedding:
         else:
             if scaling is not None:
                 raise ValueError("RotaryEmbedding: give inv_freq or scaling, not both")
-            freq, factor = torch.as_tensor(inv_freq).detach().double(), 1.0
+            freq, factor = torch.as_tensor(inv_freq).detach().to(torch.float64, copy=True), 1.0  # (the caller may reuse theirs)
             if tuple(freq.shape) != (rotary_dim // 2,):
                 raise ValueError(f"RotaryEmbedding: inv_freq must have shape ({rotary_dim // 2},), got {tuple(freq.shape)}")
         self.head_dim, self.rotary_dim, self.layout = int(head_dim), rotary_dim, layout
@@ -194,7 +194,7 @@ class RotaryEmbedding:
     @property
     def inv_freq(self) -> torch.Tensor:
         """Angle per position of each pair, float64 on the host."""
-        return self._freq.cpu()
+        return self._freq.to("cpu", copy=True)
 
     def _turns_on(self, device: torch.device) -> int:
         """The table's address on ``device``."""
