@@ -46,6 +46,14 @@ _SCALING_KEYS = {
 _NO_EFFECT = {"rope_type", "type", "rope_theta", "original_max_position_embeddings", "max_position_embeddings", "finetuned"}
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the stretches of memory from the first to the last element of ``a`` and ``b`` meet."""
+    if not (a.numel() and b.numel()):
+        return False
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
 def rotary_frequencies(rotary_dim: int, base: float | None = None, scaling: dict | None = None) -> tuple[torch.Tensor, float]:
     """Angle per position of each of the ``rotary_dim / 2`` pairs (float64, on the host) and the
     factor on sine and cosine.
@@ -321,8 +329,8 @@ class RotaryEmbedding:
         """Turn ``q [B,H_q,S,D]`` and ``k [B,H_kv,S,D]`` in one launch, writing the turned keys and
         ``v [B,H_kv,S,D]`` to rows ``[tok_offset, tok_offset + S)`` of ``k_res / v_res [B,H_kv,cap,D]``
         (the exact window of a KIVI cache: the rotating form of ``kernels.kivi_append``); returns the
-        turned queries. The other rows stay as they are. Inputs must not share memory with
-        ``k_res`` / ``v_res``. Not differentiable."""
+        turned queries. The other rows stay as they are. Inputs must not lie within the memory that
+        ``k_res`` / ``v_res`` span. Not differentiable."""
         fn = "RotaryEmbedding.append"
         self._check_append(q, k, v)
         B, H, S, D = k.shape
@@ -345,7 +353,9 @@ class RotaryEmbedding:
             raise ValueError(f"{fn}: k_res and v_res must be different memory")
         held = (k_res.untyped_storage().data_ptr(), v_res.untyped_storage().data_ptr())
         if q.untyped_storage().data_ptr() in held or k.untyped_storage().data_ptr() in held or v.untyped_storage().data_ptr() in held:
-            raise ValueError(f"{fn}: q, k and v must not share memory with k_res / v_res")
+            # (one storage: views of different parts of it are fine)
+            if any(_overlap(x, t) for x in (q, k, v) for t in (k_res, v_res)):
+                raise ValueError(f"{fn}: q, k and v must not share memory with k_res / v_res")
         out = _empty(q)
         es = k.element_size()
         ks, vs = k_res.stride(), v_res.stride()
