@@ -52,6 +52,8 @@ class KiviRows:
         if first.ndim != 4:
             raise ValueError(f"{fn}: {tensors[0][0]} must be 4D, got {tuple(first.shape)}")
         B, H = first.shape[:2]
+        if H < 1:
+            raise ValueError(f"{fn}: at least one kv head expected, got {tuple(first.shape)}")
         D = k_res.shape[-1] if k_res is not None else k_codes.shape[3] * 8 // store_bits
         if D not in (64, 128):
             raise ValueError(f"{fn}: head_dim={D} must be 64 or 128")
