@@ -623,8 +623,10 @@ typedef struct vq_kivi_rows {
 /* out[b, h, r] = softmax(scale * q[b, h, r] . [K_prefix | K_own[b]]) . [V_prefix | V_own[b]] with
  * kv head h / (H_q/H_kv). The prefix is ONE store read by all B requests; every query row sees all
  * of it. Own slot t of request b (packed tokens first, then the exact rows; n = n_quant + n_res of
- * `own`) is seen by query row r when t >= own_start[b] (NULL: 0; slots before it are padding) and,
- * with VQ_ATTEND_CAUSAL, t <= n - S_q + r. A row that sees nothing gives zeros (and lse -inf).
+ * `own`) is seen by query row r when t >= own_start[b] (NULL: 0; slots before it are padding: their values, exact
+ * rows and key groups of padding alone may hold anything, but padding keys that share a packed group with live
+ * tokens set its scale and zero, so they have to be finite and of ordinary size) and,
+ * with VQ_ATTEND_CAUSAL, t <= n - S_q + r; an infinite or NaN value reaches every row of its request. A row that sees nothing gives zeros (and lse -inf).
  * float16 or bfloat16; D 64 or 128, group 32, store_bits 2, 4 or 8. Decoded keys and values
  * enter the tensor cores as float16 (also for bfloat16 queries), so scale, zero, code*scale+zero, the
  * exact rows and q must lie within +-65504, and small ones lose bits that bfloat16 would keep: a key
@@ -643,7 +645,8 @@ typedef struct vq_shared_attend_args {
     float scale;
     int32_t flags;            /* 0 or VQ_ATTEND_CAUSAL */
     vq_kivi_rows prefix, own;
-    void *workspace;          /* >= vq_kivi_shared_attend_workspace_bytes(args), 16-byte aligned */
+    void *workspace;          /* >= vq_kivi_shared_attend_workspace_bytes(args), 16-byte aligned: a float32 row of
+                                 D + 2 for each of the B*H_q*S_q output rows and split of either part */
     int64_t workspace_bytes;
     int32_t variant;          /* 0 = choose by size; 1 = warp tiles for both parts; 2 = the tcgen05 kernel for
                                  the prefix (and for own tokens with more than 32 query rows a kv head), which

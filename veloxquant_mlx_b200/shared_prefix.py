@@ -139,14 +139,17 @@ def kivi_shared_prefix_attend(q: torch.Tensor, prefix: KiviRows, own: KiviRows |
 
     Every query row sees the whole prefix. ``causal=True``: of the ``n`` own tokens row ``r`` sees the slots
     ``<= n - S_q + r``; ``causal=False``: all. ``own_start`` (``int32 [B]`` on the device): own slots before
-    ``own_start[b]`` are padding and are not seen, whatever they hold (a batch padded on the left). A row
-    that sees nothing gives zeros and ``lse`` -inf.
+    ``own_start[b]`` are padding and are not seen (a batch padded on the left). Their values, exact rows and key groups
+    of padding alone may hold anything; padding keys that share a packed group of 32 with live tokens set its scale
+    and zero and have to be finite and of ordinary size. A row that sees nothing gives zeros and ``lse`` -inf. An
+    infinite or NaN value reaches every row of its request, seen or hidden by ``causal``.
 
     The prefix is read once for all query rows of a kv head. Decoded keys and values, the exact rows and q
     enter the tensor cores as float16 also for bfloat16 (so they must lie within +-65504; small ones keep 2^-25 absolute, and
     decoded bfloat16 ones of 2 and 4 bits 2^-20: bfloat16 values below about 2^-12 lose accuracy, 1.3 % at 1e-5, 14 % at
     1e-6), softmax and sums are float32. ``variant`` 1 / 2 force the warp-tile / the tensor-memory kernel for the prefix (2: ``scale`` > 0). Not
-    differentiable: tensors that carry a derivative (either mode) are refused.
+    differentiable: tensors that carry a derivative (either mode) are refused. A call takes ``4 (D + 2)`` bytes for
+    each output row and split of either part from torch's allocator (at least two: 68 MB for 65,536 rows of 128).
     """
     fn = "kivi_shared_prefix_attend"
     if q.ndim != 4:
@@ -253,7 +256,9 @@ class SharedPrefixKIVICache(StandaloneProtocol):
 
     def set_own_start(self, own_start) -> None:
         """Number of padding tokens at the front of each request's own tokens (a sequence of ``batch`` ints >= 0,
-        or None): they take slots but are never seen, and positions count from the first token after them."""
+        or None): they take slots but are never seen, and positions count from the first token after them. Their
+        keys go through the quantizer: they have to be finite and of ordinary size (see
+        :func:`kivi_shared_prefix_attend`). It stays set over :meth:`reset` and :meth:`trim`."""
         if own_start is None:
             self._start_host = self._start = None
             return
