@@ -148,7 +148,7 @@ extern "C" int32_t vq_rotary(const vq_rotary_args *args, void *stream) {
     VQ_REQUIRE(args != nullptr, VQ_ERR_SHAPE, "vq_rotary: args is NULL");
     const vq_rotary_args &a = *args;
     VQ_REQUIRE(a.dtype >= 0 && a.dtype <= 2, VQ_ERR_DTYPE, "vq_rotary: unknown dtype %d", a.dtype);
-    VQ_REQUIRE(a.B >= 0 && a.S >= 0 && a.S < (1ll << 31) && a.D >= 2 && a.D <= 65536, VQ_ERR_SHAPE, "vq_rotary: bad sizes (B=%lld, S=%lld, D=%d)",
+    VQ_REQUIRE(a.B >= 0 && a.B < (1ll << 31) && a.S >= 0 && a.S < (1ll << 31) && a.D >= 2 && a.D <= 65536, VQ_ERR_SHAPE, "vq_rotary: bad sizes (B=%lld, S=%lld, D=%d)",
                (long long)a.B, (long long)a.S, a.D);
     VQ_REQUIRE(a.rotary_dim >= 2 && a.rotary_dim <= a.D && a.rotary_dim % 2 == 0, VQ_ERR_SHAPE,
                "vq_rotary: rotary_dim=%d must be even and in 2..D=%d", a.rotary_dim, a.D);
@@ -186,6 +186,7 @@ extern "C" int32_t vq_rotary(const vq_rotary_args *args, void *stream) {
     VQ_REQUIRE(total < (1 << 24), VQ_ERR_SHAPE, "vq_rotary: too many heads (%lld)", (long long)total);
     const int64_t n_tok = a.B * a.S;
     if (n_tok == 0 || total == 0) return VQ_OK;
+    VQ_REQUIRE(n_tok < (1ll << 38), VQ_ERR_SHAPE, "vq_rotary: too many tokens (%lld)", (long long)n_tok);  // (more than a launch's threads)
     DeviceInfo di;
     int32_t rc = device_info(&di);
     if (rc != VQ_OK) return rc;
@@ -214,8 +215,8 @@ extern "C" int32_t vq_rotary(const vq_rotary_args *args, void *stream) {
     const int64_t fill = (int64_t)di.sm_count * 1024;
     const int64_t lanes = std::min<int64_t>(total, std::max<int64_t>(ceil_div(total, 12), ceil_div(fill, n_tok * p.units)));
     p.head_lanes = (int)lanes;
+    VQ_REQUIRE((double)n_tok * p.units * (double)lanes < (double)(1ll << 31) * (kThreads - 1), VQ_ERR_SHAPE, "vq_rotary: too many tokens (%lld)", (long long)n_tok);
     const int64_t blocks = ceil_div(n_tok * p.units * lanes, kThreads);
-    VQ_REQUIRE(blocks < (1ll << 31), VQ_ERR_SHAPE, "vq_rotary: too many tokens (%lld)", (long long)n_tok);
     cudaStream_t st = (cudaStream_t)stream;
     const bool il = a.layout == 1;
     const unsigned nb = (unsigned)blocks;

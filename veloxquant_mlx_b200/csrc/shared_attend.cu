@@ -632,7 +632,7 @@ int32_t validate(const vq_shared_attend_args &a) {
     VQ_REQUIRE(a.store_bits == 2 || a.store_bits == 4 || a.store_bits == 8, VQ_ERR_SHAPE, "%s: store_bits=%d must be 2, 4 or 8", fn, a.store_bits);
     VQ_REQUIRE((a.flags & ~VQ_ATTEND_CAUSAL) == 0 && a.variant >= 0 && a.variant <= 2 && a.n_splits >= 0, VQ_ERR_SHAPE,
                "%s: unknown flags (%d), variant (%d) or n_splits (%d)", fn, a.flags, a.variant, a.n_splits);
-    VQ_REQUIRE((int64_t)a.B * a.H_q * a.S_q < (1ll << 31), VQ_ERR_SHAPE, "%s: too many query rows", fn);
+    VQ_REQUIRE((int64_t)a.B * a.H_q < (1ll << 31) && (int64_t)a.B * a.H_q * a.S_q < (1ll << 31), VQ_ERR_SHAPE, "%s: too many query rows", fn);
     VQ_REQUIRE(a.q && a.out, VQ_ERR_SHAPE, "%s: q/out is NULL", fn);
     VQ_REQUIRE(is_aligned(a.q, 16) && is_aligned(a.out, 16), VQ_ERR_ALIGN, "%s: q and out must be 16-byte aligned", fn);
     for (const vq_kivi_rows *s : {&a.prefix, &a.own}) {
