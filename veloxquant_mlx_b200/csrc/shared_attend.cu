@@ -109,7 +109,7 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
     constexpr int ROWS = 8 * NT;
     constexpr float BASE = Codes<SB>::kBase;
     // codes through half precision (half_codes); a lane's channels 8 j + i of K then pair with 8 j + i + 4
-    constexpr bool HALF = std::is_same<T, __nv_bfloat16>::value && SB != 8;
+    constexpr bool HALF = kHalfDecode<SB, T>;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float sh_m[kWarps][ROWS], sh_l[kWarps][ROWS];
     let_next_start();

@@ -1,6 +1,7 @@
 // Internal interface between the shared-prefix attention's entry point and its prefix kernel.
 #pragma once
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -100,6 +101,8 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
 // bfloat16's own rounding), 0.0023 / 0.013 / 0.14 around 1e-4 / 1e-5 / 1e-6 (0.0017 / 0.0022 / 0.018). The contract in
 // vqb200.h says so. float16 data keeps the float32 form: there the three roundings would show (its own is 0.0002).
 // `w8` is w >> 8; pair i (0..3) is the codes in bits SB*i of the two halves of w.
+template <int SB, typename T>
+constexpr bool kHalfDecode = std::is_same<T, __nv_bfloat16>::value && SB != 8;
 template <int SB>
 __device__ __forceinline__ uint32_t half_codes(uint32_t w, uint32_t w8, int i) {
     const int bit = SB == 2 ? 2 * i : 4 * (i & 1);

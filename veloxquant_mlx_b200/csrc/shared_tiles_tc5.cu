@@ -177,14 +177,17 @@ struct TileParams {
 };
 
 // The block is launched with 96 registers a thread; where decoding needs fewer, the two softmax warpgroups
-// take over what the two decoding ones can spare (their sum is what the four were launched with).
+// take over what the two decoding ones can spare (their sum is what the four were launched with: a kernel compiled to
+// fewer would wait for registers that nobody gives back, so the launch looks at the count).
+constexpr int kLaunchRegisters = 96, kMore = 120, kFewer = 72;
+static_assert(kMore + kFewer <= 2 * kLaunchRegisters, "two warpgroups take what the two others give");
 template <bool SPARE>
 __device__ __forceinline__ void more_registers() {
-    if constexpr (SPARE) asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
+    if constexpr (SPARE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMore));
 }
 template <bool SPARE>
 __device__ __forceinline__ void fewer_registers() {
-    if constexpr (SPARE) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if constexpr (SPARE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewer));
 }
 
 template <int D>
@@ -237,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
     using L = Layout<D>;
     constexpr int CHUNKS = D / 8;      // 8-channel chunks of a row
     constexpr int RB = D * SB / 8;     // bytes of a packed row
-    constexpr bool HALF = std::is_same<T, __nv_bfloat16>::value && SB != 8;  // decode8_half; channels of a chunk spread
+    constexpr bool HALF = kHalfDecode<SB, T>;  // decode8_half; channels of a chunk spread
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -726,6 +729,13 @@ int32_t launch(const TileParams &p, unsigned blocks, cudaStream_t st) {
     static std::atomic<uint64_t> allowed{0};
     const int32_t rc = allow_shared_memory(&shared_tiles_tc5_kernel<D, SB, T>, Layout<D>::BYTES, allowed);
     if (rc != VQ_OK) return rc;
+    if constexpr (kHalfDecode<SB, T>) {
+        static const int registers = [] {
+            cudaFuncAttributes at;
+            return cudaFuncGetAttributes(&at, &shared_tiles_tc5_kernel<D, SB, T>) == cudaSuccess ? at.numRegs : 0;
+        }();
+        VQ_REQUIRE(registers >= kLaunchRegisters, VQ_ERR_CUDA, "shared_tiles_tc5_kernel: compiled to %d registers, its warps share %d", registers, kLaunchRegisters);
+    }
     int dev = 0;
     VQ_CHECK_CUDA(cudaGetDevice(&dev));
     if (!(g_launched.load(std::memory_order_relaxed) & device_bit(dev))) g_launched.fetch_or(device_bit(dev));
