@@ -238,7 +238,8 @@ class RotaryEmbedding:
         self._check(fn, q, k)
         if v.shape != k.shape or v.dtype is not k.dtype or v.device != k.device:
             raise ValueError(f"{fn}: v {tuple(v.shape)} {v.dtype} must be like k {tuple(k.shape)} {k.dtype}")
-        if _lib.carries_derivative(q, k, v):
+        if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or (
+                forward_ad._current_level >= 0 and _lib.carries_derivative(q, k, v)):
             raise ValueError(f"{fn}: not differentiable; rotate and append to the cache separately, or call it under torch.no_grad()")
 
     @staticmethod
