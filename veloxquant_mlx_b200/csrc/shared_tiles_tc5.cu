@@ -22,8 +22,8 @@
 // the exponent, and leaves with m. That S of step i + 1 is complete implies that P V of step i is (MMAs of one thread
 // complete in order), so only the second half of a tile waits for more (P V of the first).
 //
-// Measured at 4 bits in bfloat16: 256 query rows of each of 8 kv heads behind 32K tokens, 18 splits, 50 us; 8192 rows
-// behind 8K tokens, 340 us = 0.82 PFLOP/s, 49 % of the measured bfloat16 rate. A pair of row tiles takes
+// Measured at 4 bits in bfloat16: 256 query rows of each of 8 kv heads behind 32K tokens, 13 splits (104 CTAs, beside
+// the own tokens' kernel), 56-60 us; 8192 rows behind 8K tokens, 337 us = 0.83 PFLOP/s, 50 % of the measured bfloat16 rate. A pair of row tiles takes
 // about 4300 clocks a token tile, against 2048 for the MMAs, 2048 for the exponentials (16 a clock), 1000 for
 // HBM and about 2400 of instruction issue: what bounds it is the chain of one stream (1000 until scores are
 // there: the last half of P V 256, Q K 700; weights 3350, of which about 2000 beside the other stream's), of
