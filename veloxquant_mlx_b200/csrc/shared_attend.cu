@@ -21,9 +21,10 @@ constexpr int kGroup = 32;
 constexpr int kExact = 12;  // exact rows of one work item: as many bytes as a packed group of 4-bit codes
 constexpr int kWarps = 4;
 constexpr int kStages = 2;
-// Weights, at most 1, are held times 2^15: float16's smallest step then is 2^-39 of the row's largest weight
-// instead of 2^-24, so that many tokens behind one that outweighs them are not lost. The factor is in the exponent.
-constexpr float kLift = 15.f;
+// Weights, at most 1, are held times 2^7: float16's smallest step then is 2^-31 of the row's largest weight instead
+// of 2^-24, so that many tokens behind one that outweighs them are not lost. The factor is in the exponent: the
+// running maximum m is held 7 lower (8 at most where float32 rounds it; 15 could become 16, and 2^16 is no float16).
+constexpr float kLift = 7.f;
 
 struct RowsParams {
     const void *q;
@@ -239,7 +240,7 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
                 for (int k = 0; k < STEPS; ++k)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        s[nt][k][c] *= p.scale_log2;
+                        s[nt][k][c] = __fmul_rn(s[nt][k][c], p.scale_log2);  // (rounded here: the maximum and the weights see the same)
                         mx[c & 1] = fmaxf(mx[c & 1], s[nt][k][c]);
                     }
             } else {
@@ -248,19 +249,18 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const int slot = slot0 + 16 * k + 8 * (c >> 1) + tau;
-                        s[nt][k][c] = slot >= first_slot && slot < min(lim[nt][c & 1], end) ? s[nt][k][c] * p.scale_log2 : -INFINITY;
+                        s[nt][k][c] = slot >= first_slot && slot < min(lim[nt][c & 1], end) ? __fmul_rn(s[nt][k][c], p.scale_log2) : -INFINITY;
                         mx[c & 1] = fmaxf(mx[c & 1], s[nt][k][c]);
                     }
             }
-            float low[2], f[2];
+            float base[2], f[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], d));
-                const float mn = fmaxf(m[nt][i], mx[i]);
-                const float base = mn == -INFINITY ? 0.f : mn;
-                f[i] = ex2(m[nt][i] - base);
-                low[i] = base - kLift;
+                const float mn = fmaxf(m[nt][i], mx[i] - kLift);
+                base[i] = mn == -INFINITY ? 0.f : mn;
+                f[i] = ex2(m[nt][i] - base[i]);
                 m[nt][i] = mn;
                 l[nt][i] *= f[i];
             }
@@ -273,7 +273,7 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
                 float e[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    e[c] = ex2(s[nt][k][c] - low[c & 1]);
+                    e[c] = ex2(s[nt][k][c] - base[c & 1]);
                     l[nt][c & 1] += e[c];
                 }
                 pb[nt][k][0] = transpose8x8(pack_f16(e[0], e[1]));
@@ -454,7 +454,7 @@ shared_attend_rows_kernel(const __grid_constant__ RowsParams p) {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], d);
             const int r = 8 * nt + 2 * c4 + i;
-            if (g8 == 0) { sh_m[warp][r] = m[nt][i] - kLift; sh_l[warp][r] = l[nt][i]; }  // (l and o are 2^kLift times those of m)
+            if (g8 == 0) { sh_m[warp][r] = m[nt][i]; sh_l[warp][r] = l[nt][i]; }
             float *dst = sh_o + (warp * ROWS + r) * LD + g8 * CN;
 #pragma unroll
             for (int j = 0; j < MT; ++j) *reinterpret_cast<float2 *>(dst + 2 * j) = make_float2(o[nt][j][i], o[nt][j][2 + i]);

@@ -19,7 +19,7 @@
 // the tokens before, is then rescaled by the row's own thread. Weights are held times 2^7: up to 2^15, which float16
 // holds, and down to 2^-32 of 2^m before its smallest step (2^-25 without the factor, and then the tail behind one
 // token that outweighs all others is lost: 4096 tokens of 2^-26 each came out as 0). The factor costs nothing: it is in
-// the exponent, and leaves with m. That S of step i + 1 is complete implies that P V of step i is (MMAs of one thread
+// the exponent (m itself is held 7 lower, so that rescaling stays exact). That S of step i + 1 is complete implies that P V of step i is (MMAs of one thread
 // complete in order), so only the second half of a tile waits for more (P V of the first).
 //
 // Measured at 4 bits in bfloat16: 256 query rows of each of 8 kv heads behind 32K tokens, 13 splits (104 CTAs, beside
@@ -45,6 +45,7 @@ constexpr int kThreads = 17 * 32;
 constexpr uint32_t kSpin = 1u << 20;
 constexpr float kLazy = 8.f;       // log2 of how far a maximum may rise before O is rescaled
 constexpr float kLift = 7.f;       // log2 of the factor on weights: kLazy + kLift = 15, below float16's 2^16
+constexpr float kFar = 1 << 20;    // scores (base 2) from here on are spaced by 2^-3 and more
 
 __device__ int g_shared_timeout = 0;
 std::atomic<uint64_t> g_launched{0};  // one bit a device that the kernel was ever launched on (or captured for)
@@ -334,7 +335,8 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
         const int lim = is_prefix || !p.causal ? n_slots : n_slots - p.S_q + r % p.S_q + 1;
         // (tiles within [first_slot, the warp's smallest lim) need no mask)
         const int all_see = __reduce_min_sync(0xffffffffu, lim);
-        float m = -INFINITY, l = 0.f;  // reference maximum (times scale, base 2) and the weights' sum
+        float m = -INFINITY, l = 0.f;  // reference maximum (times scale, base 2) less kLift, and the weights' sum
+        bool far = false;              // (of the whole warp) a maximum lies far from 0
         for (int i = 0; i < n_mine; ++i) {
             const int t = t_lo + (two ? i : 2 * i + s);
             const int slot0 = t < tiles_packed ? t * kTile : st.n_quant + (t - tiles_packed) * kTile;
@@ -377,10 +379,11 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
             for (int c = 0; c < kTile; c += 64) {  // half of the tokens: their largest score may first raise m
                 tmem_ld_wait(v);
                 tmem_ld_wait(w);
-                const float m0 = largest(c, v), mx = fmaxf(m0, largest(c + 32, w)) * p.scale_log2;
-                if (__any_sync(0xffffffffu, mx > m + kLazy)) {
-                    const float mn = mx > m + kLazy ? mx : m, f = m == -INFINITY ? 0.f : mn == m ? 1.f : ex2(m - mn);
+                const float m0 = largest(c, v), mx = __fmul_rn(fmaxf(m0, largest(c + 32, w)), p.scale_log2);
+                if (__any_sync(0xffffffffu, mx - m > kLazy + kLift)) {  // (a difference: exact however large the two are)
+                    const float mn = mx - m > kLazy + kLift ? mx - kLift : m, f = m == -INFINITY ? 0.f : mn == m ? 1.f : ex2(m - mn);
                     m = mn;
+                    far = __any_sync(0xffffffffu, m != -INFINITY && fabsf(m) > kFar);
                     l *= f;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) { sum[k].x *= f; sum[k].y *= f; }
@@ -392,7 +395,18 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
                         for (int k = 0; k < D; k += 8) scale_o(to + k, f);
                     }
                 }
-                base = m == -INFINITY ? 0.f : kLift - m;
+                base = m == -INFINITY ? 0.f : -m;
+                if (far) {
+                    // There the product that the fused multiply-add does not round exceeds the rounded maximum by half
+                    // a step of float32, more than the weights have room for: products are rounded first here.
+                    const float back = 1.f / p.scale_log2;
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        v[k] = (__fmul_rn(v[k], p.scale_log2) + base) * back;
+                        w[k] = (__fmul_rn(w[k], p.scale_log2) + base) * back;
+                    }
+                    base = 0.f;
+                }
                 weights(c, v);
                 if (c == 0) tmem_ld32(ts + 64, v);
                 weights(c + 32, w);
@@ -404,7 +418,6 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tiles_tc5_kernel(const __g
             }
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         }
-        m -= kLift;  // (O and l are 2^kLift times those of m)
         // O goes out through shared memory: a row a lane there, whole rows at a time to global memory. The
         // tiles it overwrites are done with when both streams are.
         if (n_steps > 0) wait(kODone, 0);
