@@ -164,7 +164,7 @@ class RotaryEmbedding:
     (``torch.autograd.forward_ad``), not through positions or frequencies.
 
     The frequency table is put on a device at its first use there; make that use (or pass
-    ``device=``) before a CUDA-graph capture. Where a backward pass is captured, PyTorch's own rule
+    ``device=``) before a CUDA-graph capture. Copies and pickles keep the tables that lie on their device. Where a backward pass is captured, PyTorch's own rule
     holds: no graph that an earlier eager pass built over the same leaves may still be alive.
     """
 
@@ -198,6 +198,11 @@ class RotaryEmbedding:
             device = freq.device
         if device is not None:
             self._turns_on(torch.device(device))
+
+    def __setstate__(self, state) -> None:
+        # (a load may have put the tables elsewhere than on the device they are for: those are made anew at their next use)
+        turns = {i: t for i, t in state["_turns"].items() if t.is_cuda and t.device.index == i}
+        self.__dict__.update(state, _turns=turns)
 
     @property
     def inv_freq(self) -> torch.Tensor:
