@@ -638,7 +638,7 @@ class KIVIKVCache(StandaloneProtocol):
         g = self._group_size
         B, H, _, D = src_k.shape
         s0, s1, s2, s3 = src_k.stride()
-        if (src_k.is_cuda and src_k.dtype is src_v.dtype and src_k.shape == src_v.shape and src_v.stride() == (s0, s1, s2, s3)
+        if (src_k.is_cuda and self._k_codes.device == src_k.device and src_k.dtype is src_v.dtype and src_k.shape == src_v.shape and src_v.stride() == (s0, s1, s2, s3)
                 and s3 == 1 and s2 == D and (B == 1 or s0 == H * s1) and n_flush > 0
                 and self._n_quantized + n_flush <= self._cap and self._n_quantized % g == 0):
             # Evenly spaced (batch, head) slabs of whole rows, into this cache's own buffers: the two
